@@ -27,6 +27,8 @@ PROTOTYPES = {
     "attn_b200_rope_inplace": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i64, _i32, _vp, _vp]),
     "attn_b200_rope_write_kv": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i64,
                                        _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "attn_b200_qk_norm_rope": (_i32, [_vp] * 13 + [_i64, _i32, _i32, _i32, _i32] + [_i64] * 7 + [_f32] + [_i32] * 4 +
+                               [_vp] * 4),
     "attn_b200_paged_decode": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _i64,
                                       _i32, _i32, _i32, _i32, _i64, _i64, _i32, _i32, _i32, _i32, _f32, _vp, _vp,
                                       _i32, _i32, _i32, _vp, _vp]),

@@ -153,6 +153,163 @@ def rope_and_cache_write(Q, K, V, positions, cos, sin, slots, K_cache, V_cache, 
 
 
 # ----------------------------------------------------------------------------------------------
+# norm of every query and key head with the rotation (and the cache append) in one pass
+# ----------------------------------------------------------------------------------------------
+def _check_on(dev: torch.device, *tensors) -> None:
+    """``(tensor or None, name)`` pairs: CUDA tensors of one device (contiguity is the caller's business)."""
+    for x, name in tensors:
+        if x is None:
+            continue
+        if not isinstance(x, torch.Tensor) or not x.is_cuda:
+            raise RuntimeError(f"{name} must be a CUDA tensor")
+        if x.device != dev:
+            raise RuntimeError(f"{name} must be on the same device as Q ({dev}), not on {x.device}")
+
+
+def _flag_word(x) -> None:
+    if x is not None and (x.dtype != torch.int32 or x.numel() < 1):
+        raise RuntimeError("err_flag must be an int32 tensor with one entry")
+
+
+def _rows(x, name: str) -> None:
+    """A matrix of whole rows: contiguous columns, rows any non-negative distance apart that keeps them disjoint."""
+    if x.dim() != 2 or (x.size(1) > 1 and x.stride(1) != 1) or (x.size(0) > 1 and x.stride(0) < x.size(1)):
+        raise RuntimeError(f"{name} must be two-dimensional with contiguous rows that do not overlap")
+
+
+def _kv_scales(kvd: int, k_scale, v_scale, hkv: int, dev) -> None:
+    if kvd != _lib.E4M3:
+        return
+    if k_scale is None or v_scale is None:
+        raise RuntimeError("FP8 KV needs k_scale and v_scale (float32 [Hkv])")
+    _check_on(dev, (k_scale, "k_scale"), (v_scale, "v_scale"))
+    for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        if t.dtype != torch.float32 or t.numel() != hkv or not t.is_contiguous():
+            raise RuntimeError(f"{n} must be contiguous float32 [Hkv]")
+
+
+def _span(x):
+    return x.data_ptr(), x.data_ptr() + ((x.size(0) - 1) * x.stride(0) + x.size(1)) * x.element_size()
+
+
+def _may_overlap(a, b) -> bool:
+    """Whether two row matrices can share memory.  Matrices with one row distance (slices of one
+    buffer) are compared by their columns, all others by their whole extent."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    step = a.stride(0) * a.element_size()
+    if a.size(0) == 1 or b.size(0) == 1 or step != b.stride(0) * b.element_size():
+        return True
+    gap = (b0 - a0) % step
+    return gap < a.size(1) * a.element_size() or gap + b.size(1) * b.element_size() > step
+
+
+def _qk_norm_rope(what, Q, K, V, q_weight, k_weight, positions, cos, sin, slots, K_cache, V_cache, head_dim, eps,
+                  k_scale, v_scale, out, err_flag):
+    _check_on(getattr(Q, "device", None), (Q, "Q"), (K, "K"), (V, "V"), (q_weight, "q_weight"), (k_weight, "k_weight"),
+              (positions, "positions"), (cos, "cos"), (sin, "sin"), (slots, "slots"), (K_cache, "K_cache"),
+              (V_cache, "V_cache"), (err_flag, "err_flag"))
+    _flag_word(err_flag)
+    dev, dt = Q.device, _dtype_code(Q, "Q")
+    for t, n in ((Q, "Q"), (K, "K")) + (((V, "V"),) if V is not None else ()):
+        _rows(t, n)
+        if t.dtype != Q.dtype or t.size(0) != Q.size(0):
+            raise RuntimeError("Q, K and V must share a dtype and the number of rows")
+    n_tokens = Q.size(0)
+    if head_dim <= 0 or Q.size(1) % head_dim or K.size(1) % head_dim or not Q.size(1) or not K.size(1):
+        raise RuntimeError("Q.size(1) and K.size(1) must be positive multiples of head_dim")
+    _int32(positions, "positions")
+    if positions.numel() != n_tokens:
+        raise RuntimeError("positions must have one entry per row of Q")
+    for t, n in ((cos, "cos"), (sin, "sin"), (q_weight, "q_weight"), (k_weight, "k_weight")):
+        _check_input(t, n)
+    if cos.dim() != 2 or sin.shape != cos.shape or 2 * cos.size(1) > head_dim:
+        raise RuntimeError("cos and sin must be [max_pos, rot_half] with 2 * rot_half <= head_dim")
+    if q_weight.numel() != head_dim or k_weight.numel() != head_dim:
+        raise RuntimeError("q_weight and k_weight must have head_dim entries")
+    if cos.dtype != sin.dtype or cos.dtype not in (Q.dtype, torch.float32):
+        raise RuntimeError("cos and sin must both have Q's dtype or both be float32")
+    if q_weight.dtype != k_weight.dtype or q_weight.dtype not in (Q.dtype, torch.float32):
+        raise RuntimeError("q_weight and k_weight must both have Q's dtype or both be float32")
+    if not eps >= 0:
+        raise RuntimeError("eps must not be negative")
+    hk, kvd, n_slots = K.size(1) // head_dim, dt, 0
+    if slots is not None:
+        _int32(slots, "slots")
+        if slots.numel() != n_tokens:
+            raise RuntimeError("slots must have one entry per row of Q")
+        _check_input(K_cache, "K_cache")
+        _check_input(V_cache, "V_cache")
+        kvd, n_slots = _kv_code(K_cache, Q), K_cache.size(0)
+        if V.shape != K.shape or K_cache.dim() != 2 or K_cache.size(1) != K.size(1) or V_cache.shape != K_cache.shape:
+            raise RuntimeError("V must match K, and the pools must be [slots, Hk*head_dim]")
+        if V_cache.dtype != K_cache.dtype:
+            raise RuntimeError("K_cache and V_cache must share a dtype")
+        _kv_scales(kvd, k_scale, v_scale, hk, dev)
+    if out is None:
+        # contiguous whatever the inputs' strides are: what the attention operators take
+        Qo = torch.empty(n_tokens, Q.size(1), dtype=Q.dtype, device=dev)
+        Ko = torch.empty(n_tokens, K.size(1), dtype=Q.dtype, device=dev)
+    else:
+        Qo, Ko = out
+        _check_on(dev, (Qo, "out[0]"), (Ko, "out[1]"))
+        for t, x, n in ((Qo, Q, "out[0]"), (Ko, K, "out[1]")):
+            _rows(t, n)
+            if t.shape != x.shape or t.dtype != x.dtype:
+                raise RuntimeError(f"{n} must have the shape and dtype of its input")
+            for y in (Q, K, V):
+                same = y is x and t.data_ptr() == x.data_ptr() and (t.stride(0) == x.stride(0) or n_tokens <= 1)
+                if y is not None and not same and _may_overlap(t, y):
+                    raise RuntimeError(f"{n} must be its input itself or share no memory with Q, K and V")
+        if _may_overlap(Qo, Ko):
+            raise RuntimeError("out[0] and out[1] must not share memory")
+    if n_tokens == 0:
+        return Qo, Ko
+    with _on_device(dev):
+        check(lib.attn_b200_qk_norm_rope(
+            Q.data_ptr(), K.data_ptr(), _ptr(V), Qo.data_ptr(), Ko.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
+            positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ptr(slots), _ptr(K_cache), _ptr(V_cache), n_tokens,
+            Q.size(1) // head_dim, hk, head_dim, cos.size(1), cos.size(0), n_slots, Q.stride(0), K.stride(0),
+            0 if V is None else V.stride(0), Qo.stride(0), Ko.stride(0), eps, dt, _DT[q_weight.dtype], _DT[cos.dtype], kvd,
+            _ptr(k_scale), _ptr(v_scale), _ptr(err_flag), _stream()), what)
+    return Qo, Ko
+
+
+def qk_norm_rope(Q, K, q_weight, k_weight, positions, cos, sin, head_dim: int, *, eps: float = 1e-6, out=None,
+                 err_flag: Optional[torch.Tensor] = None):
+    """RMS norm of every head of Q and K, times a weight, then the rotary embedding, in one pass (the
+    reference has the rotation only, rotary_embedding.cu:40-77).
+
+    Q ``[N, Hq*head_dim]`` and K ``[N, Hk*head_dim]`` may be column slices of one packed projection (rows any
+    distance apart); ``q_weight``/``k_weight`` ``[head_dim]`` and cos/sin ``[max_pos, rot_half]`` have Q's dtype
+    or are float32; positions int32 ``[N]``.  Per head ``x * rsqrt(mean(x^2) + eps) * weight``, then the first
+    ``2 * rot_half`` dims are rotated as by :func:`rotary_embedding_inplace`; all in 32 bits, rounded once.
+    Returns ``(Q', K')``: new contiguous tensors, or ``out=(Q', K')``, which may be Q and K themselves.
+    A token whose position is outside the table gets zeros and sets ATTN_B200_FLAG_BAD_POSITION in ``err_flag``.
+    """
+    return _qk_norm_rope("qk_norm_rope", Q, K, None, q_weight, k_weight, positions, cos, sin, None, None, None, head_dim,
+                         eps, None, None, out, err_flag)
+
+
+def qk_norm_rope_and_cache_write(Q, K, V, q_weight, k_weight, positions, cos, sin, slots, K_cache, V_cache,
+                                 head_dim: int, *, eps: float = 1e-6, k_scale=None, v_scale=None, out=None,
+                                 err_flag: Optional[torch.Tensor] = None):
+    """:func:`qk_norm_rope`, and in the same pass the append of K' and V to the KV pools at ``slots`` (int32
+    ``[N]``, distinct): :func:`rope_and_cache_write` for models that normalise queries and keys.  With
+    ``k_scale``/``v_scale`` (float32 ``[Hk]``) the pools are ``float8_e4m3fn`` and receive ``x / scale``, rounded to
+    nearest from the 32-bit value and saturated at 448.  A token whose slot is outside the pools (-1 for a
+    padding row) or whose position is outside the table is not appended and sets its bit in ``err_flag``.
+    """
+    if slots is None or V is None or K_cache is None or V_cache is None:
+        raise RuntimeError("V, slots, K_cache and V_cache must be CUDA tensors")
+    return _qk_norm_rope("qk_norm_rope_and_cache_write", Q, K, V, q_weight, k_weight, positions, cos, sin, slots, K_cache,
+                         V_cache, head_dim, eps, k_scale, v_scale, out, err_flag)
+
+
+# ----------------------------------------------------------------------------------------------
 # paged decode
 # ----------------------------------------------------------------------------------------------
 def _kv_code(kc: torch.Tensor, q: torch.Tensor) -> int:

@@ -94,6 +94,28 @@ ATTN_B200_API int attn_b200_rope_write_kv(void* q, void* k, const void* v, const
                                           int kv_dtype, const float* k_scale, const float* v_scale,
                                           int32_t* err_flag, void* stream);
 
+/* RMS norm of every query and key head, rotation and, with slots != NULL, the append to the KV pools,
+ * in one pass.  No counterpart in the reference (its rotation: rotary_embedding.cu:10-36).
+ *   q [n_tokens, n_heads_q*head_dim], k, v [n_tokens, n_heads_k*head_dim], q_out, k_out: `dtype` (F16,
+ *   BF16, F32), columns contiguous, rows *_stride elements apart (slices of one packed projection)
+ *   q_weight, k_weight [head_dim] of weight_dtype and cos, sin [max_pos, rot_half] of table_dtype: `dtype`
+ *   or F32.  2*rot_half <= head_dim; rot_half 0 (cos, sin then unused) is the norm alone.
+ * Per head  x <- x * rsqrt(mean(x^2) + eps) * weight, then the pairs (d, d + rot_half), d < rot_half, are
+ * rotated by cos/sin[positions[token]]; all in 32 bits, every stored value rounded once.
+ * q_out may be q (same stride) and k_out may be k; any other overlap is undefined.
+ * slots int32 [n_tokens] (distinct), k_cache, v_cache [n_slots, n_heads_k*head_dim] in `dtype`, or E4M3 (16-bit
+ * inputs) with k_scale, v_scale float [n_heads_k]: value rn_e4m3(x / scale), saturating.  A slot outside
+ * [0, n_slots) raises ATTN_B200_FLAG_BAD_SLOT, the token is not appended; a position outside the table
+ * raises ATTN_B200_FLAG_BAD_POSITION, the token's q_out and k_out are zero and it is not appended. */
+ATTN_B200_API int attn_b200_qk_norm_rope(const void* q, const void* k, const void* v, void* q_out, void* k_out,
+                                         const void* q_weight, const void* k_weight, const int32_t* positions,
+                                         const void* cos, const void* sin, const int32_t* slots, void* k_cache,
+                                         void* v_cache, int64_t n_tokens, int n_heads_q, int n_heads_k, int head_dim,
+                                         int rot_half, int64_t max_pos, int64_t n_slots, int64_t q_stride,
+                                         int64_t k_stride, int64_t v_stride, int64_t q_out_stride, int64_t k_out_stride,
+                                         float eps, int dtype, int weight_dtype, int table_dtype, int kv_dtype,
+                                         const float* k_scale, const float* v_scale, int32_t* err_flag, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * KV-paged single-query decode (block_size = 1 slot table).
  * Replaces paged_kv_attention_forward (paged_attention_kernel.cu:237-294, kernel :100-187) and,
