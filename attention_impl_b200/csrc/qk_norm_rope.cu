@@ -124,13 +124,41 @@ __device__ __forceinline__ bool token_ok(const NormRopeParams& p, int64_t token,
 // Vector kernel.  A head is LPH lanes; a lane owns two 16-byte chunks of every head it visits: chunk s
 // and its rotation partner s + r/N, or, beyond the rotated dims, two neighbours (the last one may be
 // alone).  Both are in registers before anything is stored, so the output may be the input.  The sum
-// of squares is log2(LPH) shuffles.  A lane keeps its place within the head, so its weights and its
-// cos/sin entries are loaded once for all heads of the token.  A token's heads are dealt to 2^tpt_log2
-// threads, kUnroll heads' loads in flight at a time.
-constexpr int kThreads = 256, kUnroll = 2;
+// of squares is log2(LPH) shuffles.  A token's heads are dealt to 2^tpt_log2 threads, kUnroll heads'
+// loads in flight at a time, the first ones before the position is known.
+//
+// A lane keeps its place within the head, so weight and rotation become four coefficients per pair,
+// formed once for the q heads and once for the k heads of the token:
+//   a' = r (a Ac - b Bs),  b' = r (b Bc + a As)   with  Ac = w_a c, Bs = w_b s, Bc = w_b c, As = w_a s
+// in packed pairs (fma.f32x2).  With the weights applied head by head the kernel was bound by instruction
+// issue.  16384 tokens, 32 + 32 heads of 128, fp16 (537 MB): 160 us then, 102 with the coefficients, 95
+// with the next round's loads ahead of the arithmetic and five CTAs per SM = 5.6 TB/s, 0.86 of the
+// measured copy rate; with the append (940 MB) 222 -> 158 us = 5.9 TB/s.
+constexpr int kThreads = 128, kUnroll = 2, kCtasPerSm = 5, kRounds = 4;
+constexpr int64_t kFillThreads = 148 * 5 * 128;
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmul.rn.f32x2 rd, ra, rb;\n\t"
+        "mov.b64 {%0, %1}, rd;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+// read once; not ld.global.nc, because the output may be the input
+__device__ __forceinline__ uint4 ld_once(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
 
 template <typename T, int LPH>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
 qk_norm_rope_kernel(const NormRopeParams p) {
     constexpr int N = Vec<T>::N;
     // a programmatic dependent (a decode kernel) may be scheduled from here on; it reads nothing this
@@ -141,90 +169,108 @@ qk_norm_rope_kernel(const NormRopeParams p) {
     const int64_t tok_raw = (int64_t)blockIdx.x * (kThreads >> p.tpt_log2) + (threadIdx.x >> p.tpt_log2);
     const bool live = tok_raw < p.n_tokens;               // whole LPH groups agree; shuffles run for all
     const int64_t token = live ? tok_raw : p.n_tokens - 1;
-    int pos;
-    int64_t slot;
-    const bool pos_ok = token_ok(p, token, live ? tid : 1, pos, slot);
 
     const int hv = p.d / N, cph = p.rot / N;
     const int sub = tid & (LPH - 1), grp = tid / LPH, ngrp = tpt / LPH;
-    // chunks of this lane (ca < 0: none; cb < 0: no second one)
-    int ca, cb;
+    // chunks of this lane (without a second one, or without any, it works on zeros and stores nothing)
     const bool rotates = sub < cph;
-    if (rotates) {
-        ca = sub;
-        cb = sub + cph;
-    } else {
-        ca = 2 * cph + 2 * (sub - cph);
-        cb = ca + 1;
-        if (ca >= hv) ca = -1;
-        if (cb >= hv) cb = -1;
-    }
-    float c[N], s[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) { c[i] = 1.f; s[i] = 0.f; }
-    if (rotates && pos_ok) {
-        load_aux<T>(p.cos, (int64_t)pos * p.rot + ca * N, p.cs_f32, c);
-        load_aux<T>(p.sin, (int64_t)pos * p.rot + ca * N, p.cs_f32, s);
-    }
-    const int heads = p.hq + p.hk;
-    const float inv_d = 1.f / (float)p.d;
-    for (int h0 = grp; h0 - grp < heads; h0 += ngrp * kUnroll) {      // the same number of rounds for every thread
-        uint4 ua[kUnroll], ub[kUnroll];
+    const int ca = rotates ? sub : 2 * cph + 2 * (sub - cph), cb = rotates ? sub + cph : ca + 1;
+    const bool has_a = ca < hv, has_b = cb < hv;
+    uint4 ua[kUnroll], ub[kUnroll];
+    auto load = [&](const T* base, int heads, int h0) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int h = h0 + u * ngrp;
+            const T* row = base + h * p.d;
             ua[u] = ub[u] = make_uint4(0, 0, 0, 0);
-            if (h < heads) {
-                const T* row = h < p.hq ? (const T*)p.q + token * p.q_stride + (int64_t)h * p.d
-                                        : (const T*)p.k + token * p.k_stride + (int64_t)(h - p.hq) * p.d;
-                if (ca >= 0) ua[u] = *reinterpret_cast<const uint4*>(row + ca * N);
-                if (cb >= 0) ub[u] = *reinterpret_cast<const uint4*>(row + cb * N);
+            if (h < heads && has_a) ua[u] = ld_once(row + ca * N);
+            if (h < heads && has_b) ub[u] = ld_once(row + cb * N);
+        }
+    };
+    const T* const q_row = (const T*)p.q + token * p.q_stride;
+    const T* const k_row = (const T*)p.k + token * p.k_stride;
+    load(q_row, p.hq, grp);
+    int pos;
+    int64_t slot;
+    const bool pos_ok = token_ok(p, token, live ? tid : 1, pos, slot);
+    float2 c[N / 2], s[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) { c[i] = make_float2(1.f, 1.f); s[i] = make_float2(0.f, 0.f); }
+    if (rotates && pos_ok) {
+        load_aux<T>(p.cos, (int64_t)pos * p.rot + ca * N, p.cs_f32, &c[0].x);
+        load_aux<T>(p.sin, (int64_t)pos * p.rot + ca * N, p.cs_f32, &s[0].x);
+    }
+    const float inv_d = 1.f / (float)p.d;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        const int heads = which ? p.hk : p.hq;
+        const T* const row = which ? k_row : q_row;
+        T* const out = which ? (T*)p.k_out + token * p.ko_stride : (T*)p.q_out + token * p.qo_stride;
+        const void* wp = which ? p.wk : p.wq;
+        float2 ac[N / 2], bs[N / 2], bc[N / 2], as[N / 2];
+        {
+            float2 wa[N / 2], wb[N / 2];
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) wa[i] = wb[i] = make_float2(0.f, 0.f);
+            if (has_a) load_aux<T>(wp, ca * N, p.w_f32, &wa[0].x);
+            if (has_b) load_aux<T>(wp, cb * N, p.w_f32, &wb[0].x);
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                ac[i] = mul2(wa[i], c[i]);
+                as[i] = mul2(wa[i], s[i]);
+                bc[i] = mul2(wb[i], c[i]);
+                bs[i] = mul2(wb[i], make_float2(-s[i].x, -s[i].y));
             }
         }
+        for (int h0 = grp; h0 - grp < heads; h0 += ngrp * kUnroll) {      // the same number of rounds for every thread
+            uint4 va[kUnroll], vb[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int h = h0 + u * ngrp;
-            const bool is_q = h < p.hq;
-            float a[N], b[N], w[N];
-            Vec<T>::unpack(ua[u], a);
-            Vec<T>::unpack(ub[u], b);
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < N; ++i) ss += a[i] * a[i] + b[i] * b[i];
-            ss = group_sum<LPH>(ss);
-            const float r = rsqrtf(ss * inv_d + p.eps);
-            if (h >= heads || !live) continue;
-            const void* wp = is_q ? p.wq : p.wk;
-            if (ca >= 0) {
-                load_aux<T>(wp, ca * N, p.w_f32, w);
-#pragma unroll
-                for (int i = 0; i < N; ++i) a[i] = a[i] * r * w[i];
+            for (int u = 0; u < kUnroll; ++u) {
+                va[u] = ua[u];
+                vb[u] = ub[u];
             }
-            if (cb >= 0) {
-                load_aux<T>(wp, cb * N, p.w_f32, w);
+            if (h0 + ngrp * kUnroll - grp < heads) load(row, heads, h0 + ngrp * kUnroll);
+            else if (!which) load(k_row, p.hk, grp);
 #pragma unroll
-                for (int i = 0; i < N; ++i) b[i] = b[i] * r * w[i];
-            }
-            if (rotates) {
+            for (int u = 0; u < kUnroll; ++u) {
+                const int h = h0 + u * ngrp;
+                float2 a[N / 2], b[N / 2];
+                Vec<T>::unpack(va[u], &a[0].x);
+                Vec<T>::unpack(vb[u], &b[0].x);
+                float2 s0 = mul2(a[0], a[0]), s1 = mul2(b[0], b[0]);
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float x = a[i], y = b[i];
-                    a[i] = x * c[i] - y * s[i];
-                    b[i] = y * c[i] + x * s[i];
+                for (int i = 1; i < N / 2; ++i) {
+                    s0 = fma2(a[i], a[i], s0);
+                    s1 = fma2(b[i], b[i], s1);
                 }
-            }
-            if (!pos_ok) {              // no such table row: the token's outputs are zero and nothing is appended
+                const float ss = group_sum<LPH>((s0.x + s0.y) + (s1.x + s1.y));
+                if (h >= heads || !live) continue;
+                const float r = rsqrtf(ss * inv_d + p.eps);
+                const float2 r2 = make_float2(r, r);
 #pragma unroll
-                for (int i = 0; i < N; ++i) a[i] = b[i] = 0.f;
-            }
-            T* out = is_q ? (T*)p.q_out + token * p.qo_stride + (int64_t)h * p.d
-                          : (T*)p.k_out + token * p.ko_stride + (int64_t)(h - p.hq) * p.d;
-            if (ca >= 0) *reinterpret_cast<uint4*>(out + ca * N) = Vec<T>::pack(a);
-            if (cb >= 0) *reinterpret_cast<uint4*>(out + cb * N) = Vec<T>::pack(b);
-            if (!is_q && slot >= 0) {
-                const int64_t at = (slot * p.hk + (h - p.hq)) * p.d;
-                if (ca >= 0) store_pool<T>(p.k_cache, at + ca * N, a, p.k_scale, h - p.hq);
-                if (cb >= 0) store_pool<T>(p.k_cache, at + cb * N, b, p.k_scale, h - p.hq);
+                for (int i = 0; i < N / 2; ++i) {
+                    const float2 x = a[i], y = b[i];
+                    a[i] = mul2(x, ac[i]);
+                    b[i] = mul2(y, bc[i]);
+                    if (rotates) {
+                        a[i] = fma2(y, bs[i], a[i]);
+                        b[i] = fma2(x, as[i], b[i]);
+                    }
+                    a[i] = mul2(a[i], r2);
+                    b[i] = mul2(b[i], r2);
+                }
+                if (!pos_ok) {              // no such table row: the token's outputs are zero and nothing is appended
+#pragma unroll
+                    for (int i = 0; i < N / 2; ++i) a[i] = b[i] = make_float2(0.f, 0.f);
+                }
+                T* o = out + h * p.d;
+                if (has_a) *reinterpret_cast<uint4*>(o + ca * N) = Vec<T>::pack(&a[0].x);
+                if (has_b) *reinterpret_cast<uint4*>(o + cb * N) = Vec<T>::pack(&b[0].x);
+                if (which && slot >= 0) {
+                    const int64_t at = (slot * p.hk + h) * p.d;
+                    if (has_a) store_pool<T>(p.k_cache, at + ca * N, &a[0].x, p.k_scale, h);
+                    if (has_b) store_pool<T>(p.k_cache, at + cb * N, &b[0].x, p.k_scale, h);
+                }
             }
         }
     }
@@ -319,9 +365,13 @@ template <typename T> int launch(const NormRopeParams& p0, cudaStream_t st) {
     if (p.d % N == 0 && p.rot % N == 0 && slots <= 32 && bits % 16 == 0 && strides % N == 0) {
         int lph = 1;
         while (lph < slots) lph <<= 1;
-        // threads per token: two rounds of kUnroll heads each, at least one LPH group, at most the CTA
+        // Threads per token: at least one LPH group, at most the CTA, and few enough that a thread makes
+        // kRounds rounds over the q heads, which pays for its coefficients (16384 tokens, 32 + 32 heads of
+        // 128, fp16: 102 us with four rounds, 109 with two, 110 with eight) - unless there are too few
+        // tokens to fill the machine that way (8 tokens: 3.7 us with one round, 7 with four).
         int tl = 0;
-        while ((1 << tl) < kThreads && ((1 << tl) < lph || (1 << tl) * 2 * kUnroll < heads * lph)) ++tl;
+        while ((1 << tl) < kThreads && ((1 << tl) < lph || (1 << tl) * kRounds * kUnroll < p.hq * lph)) ++tl;
+        while ((1 << tl) < kThreads && (1 << tl) * kUnroll < p.hq * lph && (p.n_tokens << tl) < kFillThreads) ++tl;
         p.tpt_log2 = tl;
         const int64_t per_cta = kThreads >> tl, ctas = (p.n_tokens + per_cta - 1) / per_cta;
         if (ctas > 0x7fffffff) return ATTN_B200_ETOOLARGE;
