@@ -36,6 +36,8 @@ PROTOTYPES = {
     "attn_b200_paged_decode_single_launch_ok": (_i32, [_i32, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _i32]),
     "attn_b200_paged_decode_pick_chunk": (_i32, [_i32, _i32, _i32, _i64, _i32]),
     "attn_b200_paged_decode_pick_chunk_gqa": (_i32, [_i32, _i32, _i32, _i32, _i32, _i64, _i32]),
+    "attn_b200_paged_window_decode": (_i32, [_vp] * 8 + [_i32] * 4 + [_i64] * 2 + [_i32] * 4 + [_f32, _vp, _vp, _i32, _i32, _vp,
+                                                                                          _vp]),
     "attn_b200_paged_decode_partial": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i32, _i32, _i32, _i32, _i64,
                                               _i64, _i32, _i32, _i32, _f32, _vp, _vp, _i32, _i32, _vp, _vp]),
     "attn_b200_paged_decode_static_scratch": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64,

@@ -799,6 +799,89 @@ def lse_combine(parts, Q, K=None, V=None, *, num_heads: int, scale: Optional[flo
 
 
 # ----------------------------------------------------------------------------------------------
+# sliding window with sink tokens, shared prefix
+# ----------------------------------------------------------------------------------------------
+_INT_MAX = 0x7fffffff
+
+
+def _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_scale):
+    """Checks what the single-token operators share; returns (B, D, Hkv, Q's dtype code, the pools')."""
+    for t, n in ((Q, "Q"), (K, "K"), (V, "V"), (K_cache, "K_cache"), (V_cache, "V_cache")):
+        _check_input(t, n)
+        if t.dim() != 2:
+            raise RuntimeError(f"{n} must be two-dimensional")
+    qd, kvd = _dtype_code(Q, "Q"), _kv_code(K_cache, Q)
+    if V_cache.dtype != K_cache.dtype or K.dtype != Q.dtype or V.dtype != Q.dtype:
+        raise RuntimeError("dtype mismatch between Q/K/V or K_cache/V_cache")
+    B, dim = Q.shape
+    if num_heads <= 0 or dim % num_heads or not dim:
+        raise RuntimeError("Q.size(1) must be a positive multiple of num_heads")
+    D = dim // num_heads
+    cols = K_cache.size(1)
+    if not cols or cols % D or num_heads % (cols // D) or V_cache.shape != K_cache.shape:
+        raise RuntimeError("K_cache/V_cache must be [slots, Hkv*D] with Hkv dividing num_heads")
+    if K.shape != (B, cols) or V.shape != (B, cols):
+        raise RuntimeError("K and V must be [B, Hkv*D] like the pools' rows")
+    _int32(offsets, "offsets")
+    if offsets.numel() != B:
+        raise RuntimeError("offsets must have one entry per sequence")
+    _kv_scales(kvd, k_scale, v_scale, cols // D, Q.device)
+    return B, D, cols // D, qd, kvd
+
+
+def _output(out, Q):
+    if out is None:
+        return torch.empty_like(Q)
+    _check_input(out, "out")
+    if out.shape != Q.shape or out.dtype != Q.dtype:
+        raise RuntimeError("out must have Q's shape and dtype")
+    return out
+
+
+def _window_args(window, n_sinks):
+    if int(window) != window or window < 1 or int(n_sinks) != n_sinks or n_sinks < 0:
+        raise RuntimeError("window must be a positive and n_sinks a non-negative whole number")
+    return min(int(window), _INT_MAX), min(int(n_sinks), _INT_MAX)
+
+
+def paged_window_attention_forward(Q, K, V, K_cache, V_cache, cache_indices, offsets, num_heads: int, window: int,
+                                   n_sinks: int = 0, *, scale: Optional[float] = None, k_scale=None, v_scale=None,
+                                   block_size: int = 1, out: Optional[torch.Tensor] = None,
+                                   err_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_kv_attention_forward` with a sliding window and sink tokens (not in the reference).
+
+    The current token is at position ``ctx_b`` of its sequence.  It sees itself, the ``window - 1`` cached
+    tokens before it and the first ``n_sinks`` tokens of the sequence: cached token t iff
+    ``t > ctx_b - window or t < n_sinks``.  Nothing else is read: entries of ``cache_indices`` outside the span
+    may be stale, so their pool rows can be given to other sequences.  Shapes, dtypes, grouped-query heads,
+    ``k_scale``/``v_scale`` (float8 pools) and block tables as in :func:`paged_kv_attention_forward`; a slot
+    outside the pools is skipped and sets its bit in ``err_flag``.  One kernel, no workspace.  Returns
+    O ``[B, H*D]``.
+    """
+    _check_on(getattr(Q, "device", None), (Q, "Q"), (K, "K"), (V, "V"), (K_cache, "K_cache"), (V_cache, "V_cache"),
+              (cache_indices, "cache_indices"), (offsets, "offsets"), (out, "out"), (err_flag, "err_flag"))
+    _flag_word(err_flag)
+    B, D, Hkv, qd, kvd = _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_scale)
+    window, n_sinks = _window_args(window, n_sinks)
+    _int32(cache_indices, "cache_indices")
+    max_blocks = 0
+    if block_size != 1:
+        if block_size < 1 or cache_indices.dim() != 2 or cache_indices.size(0) != B:
+            raise RuntimeError("block_size > 1 needs a block table [B, max_blocks]")
+        max_blocks = cache_indices.size(1)
+    O = _output(out, Q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    with _on_device(Q.device):
+        check(lib.attn_b200_paged_window_decode(
+            Q.data_ptr(), K.data_ptr(), V.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), cache_indices.data_ptr(),
+            offsets.data_ptr(), O.data_ptr(), B, num_heads, Hkv, D, cache_indices.numel(), K_cache.size(0), block_size,
+            max_blocks, window, n_sinks, scale, _ptr(k_scale), _ptr(v_scale), qd, kvd, _ptr(err_flag), _stream()),
+            "paged_window_attention_forward")
+    return O
+
+
+# ----------------------------------------------------------------------------------------------
 # single query over a contiguous cache
 # ----------------------------------------------------------------------------------------------
 def kv_attention_forward(Q, K, V, K_cache, V_cache, num_heads: int, *, scale: float = 1.0,

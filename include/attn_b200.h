@@ -186,6 +186,22 @@ ATTN_B200_API int attn_b200_paged_decode_pick_chunk(int B, int H, int D, int64_t
 ATTN_B200_API int attn_b200_paged_decode_pick_chunk_gqa(int B, int n_kv_heads, int group, int D, int kv_dtype,
                                                         int64_t n_tokens, int sm_count);
 
+/* Paged decode with a sliding window and sink tokens (no counterpart in the reference): as
+ * attn_b200_paged_decode, but of the ctx_b cached tokens of a sequence only those with
+ *   t > ctx_b - window  or  t < n_sinks                    (window >= 1 counts the current token itself)
+ * and the current token (k_new, v_new) take part.  Table entries and pool rows outside are not read.
+ * One kernel, no workspace; n_slots < 2^31.  An out-of-range slot is skipped (ATTN_B200_FLAG_BAD_SLOT), a
+ * sequence whose offsets are not non-decreasing or pass n_tokens (or max_blocks*block_size) counts as empty
+ * (ATTN_B200_FLAG_BAD_OFFSETS).  head_dim 64, 128, 256 with 16-bit queries run on the tensor cores, other
+ * head_dims up to 512 and F32 on the generic kernel.  `slots` has n_tokens entries (block_size 1) or is
+ * [B, max_blocks]. */
+ATTN_B200_API int attn_b200_paged_window_decode(const void* q, const void* k_new, const void* v_new, const void* k_cache,
+                                                const void* v_cache, const int32_t* slots, const int32_t* offsets,
+                                                void* out, int B, int H, int n_kv_heads, int D, int64_t n_tokens,
+                                                int64_t n_slots, int block_size, int max_blocks, int window, int n_sinks,
+                                                float scale, const float* k_scale, const float* v_scale, int q_dtype,
+                                                int kv_dtype, int32_t* err_flag, void* stream);
+
 /* Same first stage as attn_b200_paged_decode, but the second stage writes, per (b, h), one
  * partial row  [m (log2 domain), l, o[D] (un-normalised)]  of D+2 floats into
  * part_out [B, H, D+2] instead of the final output, and does NOT fold the new token.  This is
