@@ -56,6 +56,11 @@ PROTOTYPES = {
                                         _i32, _i32, _i32, _vp, _vp]),
     "attn_b200_paged_prefill": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i32, _i32, _i32, _i32, _i32,
                                        _i64, _f32, _i32, _i32, _vp, _vp]),
+    "attn_b200_paged_window_prefill": (_i32, [_vp] * 7 + [_i32, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _i32, _i32, _f32, _i32,
+                                              _i32, _vp, _vp]),
+    "attn_b200_shared_prefix_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i64, _f32, _i32, _i32]),
+    "attn_b200_shared_prefix_decode": (_i32, [_vp] * 10 + [_sz, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _f32, _vp, _vp, _i32,
+                                              _i32, _vp, _vp]),
     "attn_b200_dense_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _f32,
                                          _i32, _vp]),
 }

@@ -80,7 +80,7 @@ __device__ __forceinline__ void cluster_sync() {
 // The visible span of sequence b
 struct Span {
     int64_t beg;        // first entry of a per-token table
-    int b, first, sinks, n;
+    int b, first, sinks, n;      // n: with the shared rows, which come first
 };
 __device__ __forceinline__ Span span_of(const SpanParams& p, int b, bool report) {
     Span s;
@@ -98,14 +98,16 @@ __device__ __forceinline__ Span span_of(const SpanParams& p, int b, bool report)
     const int64_t first = ctx - p.window + 1;
     s.first = first > 0 ? (int)first : 0;
     s.sinks = p.sinks < s.first ? p.sinks : s.first;
-    s.n = s.sinks + (int)ctx - s.first;
+    s.n = p.n_prefix + s.sinks + (int)ctx - s.first;
     return s;
 }
 // pool row of the u-th visible token, or -1
 __device__ __forceinline__ int64_t slot_of(const SpanParams& p, const Span& s, int u) {
-    const int t = u < s.sinks ? u : u - s.sinks + s.first;
+    const int v = u - p.n_prefix, t = v < s.sinks ? v : v - s.sinks + s.first;
     int64_t slot;
-    if (p.block_size > 1) {
+    if (v < 0) {
+        slot = p.prefix[u];
+    } else if (p.block_size > 1) {
         const int blk = p.table[(int64_t)s.b * p.max_blocks + t / p.block_size];
         slot = blk < 0 ? -1 : (int64_t)blk * p.block_size + t % p.block_size;
     } else {
@@ -419,7 +421,7 @@ span_decode_kernel(const SpanParams p) {
 }
 
 // Any head_dim up to 32 * DPL, any type: one cluster per (sequence, query head), a warp per token, a lane
-// per dim.  Rows that the batch shares are simply visited first.  Compatibility path (fp32, odd head_dim).
+// per dim.  Compatibility path (fp32, odd head_dim).
 template <typename T, typename KV, int DPL>
 __global__ void __launch_bounds__(kWarps * 32)
 span_decode_generic_kernel(const SpanParams p) {
@@ -443,19 +445,9 @@ span_decode_generic_kernel(const SpanParams p) {
     if (threadIdx.x == 0) s_new[0] = dot * p.scale_log2;
     const float ks = p.scale_log2 * (p.k_scale ? p.k_scale[hk] : 1.f), vs = p.v_scale ? p.v_scale[hk] : 1.f;
     float m = -INFINITY, l = 0.f;
-    const int64_t total = (int64_t)p.n_prefix + sp.n;
-    for (int64_t u = rank * kWarps + warp; u < total; u += p.splits * kWarps) {
-        int64_t slot;
-        if (u < p.n_prefix) {
-            slot = p.prefix[u];
-            if (slot < 0 || slot >= p.n_slots) {
-                if (p.err_flag && lane == 0) atomicOr(p.err_flag, ATTN_B200_FLAG_BAD_SLOT);
-                continue;
-            }
-        } else {
-            slot = slot_of(p, sp, (int)(u - p.n_prefix));
-            if (slot < 0) continue;
-        }
+    for (int u = rank * kWarps + warp; u < sp.n; u += p.splits * kWarps) {
+        const int64_t slot = slot_of(p, sp, u);
+        if (slot < 0) continue;
         const KV* kr = (const KV*)p.k_cache + (slot * p.Hkv + hk) * D;
         const KV* vr = (const KV*)p.v_cache + (slot * p.Hkv + hk) * D;
         float s = 0.f, v[DPL];
@@ -557,7 +549,7 @@ int launch_generic_d(SpanParams p, int64_t span, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
     const int64_t units = (int64_t)p.B * p.H;
     int s = 1;
-    while (s < 8 && units * s < 148 * 4 && (span + p.n_prefix) > s * kWarps * 8) s *= 2;
+    while (s < 8 && units * s < 148 * 4 && span > (int64_t)s * kWarps * 8) s *= 2;
     p.splits = s;
     p.n_sets = 1;
     return launch(span_decode_generic_kernel<T, KV, DPL>, p, units, kWarps * 32 * DPL * 4, st, ready);
@@ -574,7 +566,7 @@ int launch_generic(const SpanParams& p, int64_t span, cudaStream_t st) {
 template <typename T>
 int dispatch16(const SpanParams& p, int64_t span, bool e4, cudaStream_t st) {
     const bool aligned = (((uintptr_t)p.q | (uintptr_t)p.k_new | (uintptr_t)p.k_cache | (uintptr_t)p.v_cache) & 15) == 0;
-    if (aligned && !p.prefix) {
+    if (aligned) {
         switch (p.D) {
             case 64: return e4 ? launch_mma<T, 64, true>(p, span, st) : launch_mma<T, 64, false>(p, span, st);
             case 128: return e4 ? launch_mma<T, 128, true>(p, span, st) : launch_mma<T, 128, false>(p, span, st);

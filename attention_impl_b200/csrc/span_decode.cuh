@@ -10,7 +10,7 @@ namespace attn {
 struct SpanParams {
     const void *q, *k_new, *v_new, *k_cache, *v_cache;
     const int32_t *table, *offsets;     // slot per token, or a block table; inclusive cumulative lengths
-    const int32_t* prefix;              // generic kernel only: slots of rows that every sequence sees first
+    const int32_t* prefix;              // slots of rows that every sequence sees before its own
     int n_prefix;
     void* out;
     const float* parts;                 // [n_parts, B, H, D+2] rows [o[D], m (log2 domain), l] to fold in, or null

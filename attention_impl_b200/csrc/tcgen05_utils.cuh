@@ -45,7 +45,7 @@ __device__ __forceinline__ bool mbar_test(void* bar, uint32_t parity) {
     return ok != 0;
 }
 // Bounded wait.  Returns false if the CTA is aborting or the limit ran out (then it raises the abort).
-__device__ __noinline__ void raise_timeout(AbortBox* box) {
+static __device__ __noinline__ void raise_timeout(AbortBox* box) {
     box->abort = 1;
     atomicExch(box->launch_abort, 1);
     if (box->err_flag) atomicOr(box->err_flag, ATTN_B200_FLAG_TIMEOUT);

@@ -881,6 +881,102 @@ def paged_window_attention_forward(Q, K, V, K_cache, V_cache, cache_indices, off
     return O
 
 
+def paged_window_prefill_attention(Q, K_cache, V_cache, cache_indices, kv_offsets, q_offsets, num_heads: int, window: int,
+                                   n_sinks: int = 0, *, scale: Optional[float] = None, max_q_len: Optional[int] = None,
+                                   out: Optional[torch.Tensor] = None, force_generic: bool = False,
+                                   err_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_prefill_attention` with a sliding window and sink tokens (not in the reference).
+
+    A query at position i of its sequence sees key j iff ``j <= i`` and (``j > i - window`` or
+    ``j < n_sinks``); ``window`` counts the query's own position.  Q ``[sum q_len, H*D]`` holds the last ``q_len_b``
+    tokens of every sequence, ``cache_indices``/``kv_offsets`` address all of its tokens, as in
+    :func:`paged_prefill_attention`; entries that no query of the call sees are not read and may be stale.
+    A slot outside the pools is skipped and sets its bit in ``err_flag``; a query left without any key gives
+    zeros, and so do rows of Q that belong to no sequence.  ``max_q_len`` (an upper bound of the chunk
+    lengths) avoids the one device->host sync.  float16 and bfloat16 with head_dim 64 or 128 run on the tensor
+    cores, where a non-finite value in V also reaches the queries of the same 128-row tile that do not see it;
+    every other type and head_dim up to 512 runs the generic kernel.  Returns O ``[sum q_len, H*D]``.
+    """
+    _check_on(getattr(Q, "device", None), (Q, "Q"), (K_cache, "K_cache"), (V_cache, "V_cache"), (cache_indices, "cache_indices"),
+              (kv_offsets, "kv_offsets"), (q_offsets, "q_offsets"), (out, "out"), (err_flag, "err_flag"))
+    _flag_word(err_flag)
+    for t, n in ((Q, "Q"), (K_cache, "K_cache"), (V_cache, "V_cache")):
+        _check_input(t, n)
+        if t.dim() != 2:
+            raise RuntimeError(f"{n} must be two-dimensional")
+    for t, n in ((cache_indices, "cache_indices"), (kv_offsets, "kv_offsets"), (q_offsets, "q_offsets")):
+        _int32(t, n)
+    dt = _dtype_code(Q, "Q")
+    if K_cache.dtype != Q.dtype or V_cache.dtype != Q.dtype or V_cache.shape != K_cache.shape:
+        raise RuntimeError("K_cache and V_cache must share Q's dtype and each other's shape")
+    nq, dim = Q.shape
+    if num_heads <= 0 or dim % num_heads or not dim:
+        raise RuntimeError("Q.size(1) must be a positive multiple of num_heads")
+    D, cols, B = dim // num_heads, K_cache.size(1), q_offsets.numel()
+    if not cols or cols % D or num_heads % (cols // D) or kv_offsets.numel() != B:
+        raise RuntimeError("pools must be [slots, Hkv*D] with Hkv dividing num_heads; one offset per sequence")
+    window, n_sinks = _window_args(window, n_sinks)
+    O = _output(out, Q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    with _on_device(Q.device):
+        if max_q_len is None:
+            max_q_len = max(0, int(torch.diff(q_offsets, prepend=q_offsets.new_zeros(1)).max().item())) if B else 0
+        check(lib.attn_b200_paged_window_prefill(
+            Q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), cache_indices.data_ptr(), kv_offsets.data_ptr(),
+            q_offsets.data_ptr(), O.data_ptr(), B, nq, cache_indices.numel(), min(max_q_len, nq), num_heads, cols // D, D,
+            K_cache.size(0), window, n_sinks, scale, dt, int(force_generic), _ptr(err_flag), _stream()),
+            "paged_window_prefill_attention")
+    return O
+
+
+def shared_prefix_workspace_bytes(B: int, H: int, Hkv: int, D: int, n_prefix: int, scale: float, q_dtype: int,
+                                  kv_dtype: int) -> int:
+    return lib.attn_b200_shared_prefix_workspace_bytes(B, H, Hkv, D, n_prefix, scale, q_dtype, kv_dtype)
+
+
+def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, cache_indices, offsets, num_heads: int, *,
+                                    scale: Optional[float] = None, k_scale=None, v_scale=None,
+                                    workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                                    err_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_kv_attention_forward` for a batch whose sequences all begin with the same tokens (not in the
+    reference).
+
+    ``prefix_indices`` int32 ``[P]`` are the pool rows of the shared prefix; ``cache_indices`` int32 ``[T]`` and
+    ``offsets`` int32 ``[B]`` (inclusive cumulative) those of every sequence's own cached tokens behind it, either
+    possibly empty.  The query of sequence b sees the P prefix tokens, its own tokens and the current one (K, V).
+    The prefix's K and V are read once for the batch: the query rows of all sequences are multiplied with them on
+    the tensor cores (float16/bfloat16 queries, head_dim 64 or 128, 16-bit or float8 pools).  Other types and head_dims, and
+    prefixes of at most 64 tokens, give the same result with the prefix read per sequence.  ``workspace`` (at least
+    ``shared_prefix_workspace_bytes(...)``) holds nothing between calls; two calls that may overlap need one each.
+    A slot outside the pools is skipped and sets its bit in ``err_flag``.  Returns O ``[B, H*D]``.
+    """
+    _check_on(getattr(Q, "device", None), (Q, "Q"), (K, "K"), (V, "V"), (K_cache, "K_cache"), (V_cache, "V_cache"),
+              (prefix_indices, "prefix_indices"), (cache_indices, "cache_indices"), (offsets, "offsets"), (workspace, "workspace"),
+              (out, "out"), (err_flag, "err_flag"))
+    _flag_word(err_flag)
+    B, D, Hkv, qd, kvd = _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_scale)
+    _int32(prefix_indices, "prefix_indices")
+    _int32(cache_indices, "cache_indices")
+    O = _output(out, Q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    P = prefix_indices.numel()
+    need = shared_prefix_workspace_bytes(B, num_heads, Hkv, D, P, scale, qd, kvd)
+    if workspace is None:
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
+    elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+        raise RuntimeError(f"workspace too small: {need} contiguous bytes needed")
+    with _on_device(Q.device):
+        check(lib.attn_b200_shared_prefix_decode(
+            Q.data_ptr(), K.data_ptr(), V.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), prefix_indices.data_ptr(),
+            cache_indices.data_ptr(), offsets.data_ptr(), O.data_ptr(), _ptr(workspace), need, B, num_heads, Hkv, D, P,
+            cache_indices.numel(), K_cache.size(0), scale, _ptr(k_scale), _ptr(v_scale), qd, kvd, _ptr(err_flag), _stream()),
+            "shared_prefix_attention_forward")
+    return O
+
+
 # ----------------------------------------------------------------------------------------------
 # single query over a contiguous cache
 # ----------------------------------------------------------------------------------------------

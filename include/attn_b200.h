@@ -202,6 +202,23 @@ ATTN_B200_API int attn_b200_paged_window_decode(const void* q, const void* k_new
                                                 float scale, const float* k_scale, const float* v_scale, int q_dtype,
                                                 int kv_dtype, int32_t* err_flag, void* stream);
 
+/* Decode of a batch whose sequences share a prefix (no counterpart in the reference): sequence b attends to the
+ * n_prefix pool rows prefix_slots (read once for the batch), to its own rows slots[offsets[b-1] .. offsets[b]) and
+ * to the current token.  Tensors and types as in attn_b200_paged_decode with block_size 1; n_slots and
+ * n_prefix + n_tokens < 2^31.  `workspace`: attn_b200_shared_prefix_workspace_bytes(...) bytes (0: may be NULL),
+ * 16-byte aligned, no initialisation, nothing kept between calls; not shared by calls that may overlap.
+ * A prefix of more than 64 rows with 16-bit queries, head_dim 64 or 128 and 0 < scale goes through the tensor
+ * cores, anything else (head_dim up to 512) reads the prefix per sequence.  k_scale must then be positive. */
+ATTN_B200_API size_t attn_b200_shared_prefix_workspace_bytes(int B, int H, int n_kv_heads, int D, int64_t n_prefix,
+                                                             float scale, int q_dtype, int kv_dtype);
+ATTN_B200_API int attn_b200_shared_prefix_decode(const void* q, const void* k_new, const void* v_new, const void* k_cache,
+                                                 const void* v_cache, const int32_t* prefix_slots, const int32_t* slots,
+                                                 const int32_t* offsets, void* out, void* workspace,
+                                                 size_t workspace_bytes, int B, int H, int n_kv_heads, int D,
+                                                 int64_t n_prefix, int64_t n_tokens, int64_t n_slots, float scale,
+                                                 const float* k_scale, const float* v_scale, int q_dtype, int kv_dtype,
+                                                 int32_t* err_flag, void* stream);
+
 /* Same first stage as attn_b200_paged_decode, but the second stage writes, per (b, h), one
  * partial row  [m (log2 domain), l, o[D] (un-normalised)]  of D+2 floats into
  * part_out [B, H, D+2] instead of the final output, and does NOT fold the new token.  This is
@@ -328,6 +345,20 @@ ATTN_B200_API int attn_b200_paged_prefill(const void* q, const void* k_cache, co
                                           void* out, int B, int64_t n_q_tokens, int64_t n_kv_tokens, int max_q_len,
                                           int max_kv_len, int H, int n_kv_heads, int D, int64_t n_slots, float scale,
                                           int dtype, int force_generic, int32_t* err_flag, void* stream);
+
+/* attn_b200_paged_prefill with a sliding window and sink tokens (no counterpart in the reference): the query at
+ * position i of its sequence sees key j iff j <= i and (j > i - window or j < n_sinks), window >= 1.  Slot entries
+ * that no query of the call sees are not read.  16-bit types with head_dim 64 or 128 and 0 < scale run on the
+ * tensor cores, where a non-finite V value reaches every query of a 128-row tile that has its key in a tile;
+ * head_dim up to 512 and F32 run the generic kernel.  A chunk longer than max_q_len or with bad offsets raises
+ * ATTN_B200_FLAG_BAD_OFFSETS; rows that are not computed are zero.  A key with an out-of-range slot is skipped
+ * (ATTN_B200_FLAG_BAD_SLOT). */
+ATTN_B200_API int attn_b200_paged_window_prefill(const void* q, const void* k_cache, const void* v_cache,
+                                                 const int32_t* slots, const int32_t* kv_offsets,
+                                                 const int32_t* q_offsets, void* out, int B, int64_t n_q_tokens,
+                                                 int64_t n_kv_tokens, int max_q_len, int H, int n_kv_heads, int D,
+                                                 int64_t n_slots, int window, int n_sinks, float scale, int dtype,
+                                                 int force_generic, int32_t* err_flag, void* stream);
 
 /* Dense masked attention.  Replaces naive_attention_forward (attention_kernel.cu:187-229,
  * kernel :15-94).  q, k, v, out [B, L, H*D]; mask [B, L, L] (dtype) or NULL; scores are
