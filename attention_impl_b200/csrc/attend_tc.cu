@@ -33,11 +33,25 @@ using namespace tc;
 constexpr int BM = 128, BN = 128;
 constexpr int kSub = 128 * 128;                 // bytes of a [128 rows x 64 elements] 128-byte-swizzled sub-tile
 constexpr int kStages = 2;
-constexpr int kThreads = 512;                   // softmax 0, softmax 1, {MMA thread, idle}, gather {K, K, V, V}
+constexpr int kItems = 4;                       // items published ahead
+constexpr int kThreads = 512;                   // four warpgroups: softmax 0, softmax 1, {list, MMA, Q, Q}, {K, K, V, V}
 // Registers per thread.  setmaxnreg draws on the 512 * 128 the CTA was launched with.
 template <bool E4> struct Regs {
     static constexpr int kSoftmax = E4 ? 192 : 208, kOther = E4 ? 48 : 56, kGather = E4 ? 80 : 40;
     static_assert(8 * 32 * kSoftmax + 4 * 32 * kOther + 4 * 32 * kGather <= kThreads * 128, "register pool");
+};
+
+// What the CTA works on next: a pair of query tiles and their list of keys
+struct Item {
+    int tiles, w0, n;          // key tiles (0: no more work), keys of the first tile, keys
+    int sinks, first;          // list entry u is token u < sinks ? u : u - sinks + first of the table at `beg`
+    int64_t beg;
+    int hk;
+    int jb[2], je[2];          // key tiles of each warpgroup (key_split: every second one from jb)
+    int row0[2], head[2];      // first query row (window: in the chunk) and head (window) of each query tile
+    int n_rows, shift;         // query rows of the sequence (prefix: of the KV head); window: position of row 0
+    int64_t q_beg;
+    int part;                  // prefix: first of this CTA's partial sets
 };
 
 template <int HD> struct Smem {
@@ -45,43 +59,119 @@ template <int HD> struct Smem {
     alignas(1024) unsigned char q[2][kTile];
     alignas(1024) unsigned char k[kStages][kTile];
     alignas(1024) unsigned char v[kStages][kTile];
-    alignas(16) unsigned char bad[4][BN];       // rows of a tile without a pool row (ring of four tiles)
-    alignas(8) unsigned long long q_full[2];
+    alignas(1024) unsigned char extra[2][kTile / 2];    // window: output staging; e4m3: raw K tile, raw V tile
+    alignas(16) unsigned char bad[4][BN];               // rows of a tile without a pool row (ring of four tiles)
+    signed char row_exp[2][BM];                         // bf16 queries over e4m3 rows: the power of two taken out of q
+    Item item[kItems];
+    alignas(8) unsigned long long item_full[kItems], item_empty[kItems];
+    unsigned long long q_full[2], q_empty[2], o_free[2];
     unsigned long long s_full[2], p_half[2], p_full[2], o_full[2];
     unsigned long long k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
     unsigned int tmem_base;
     int any_bad;
-    int launch_abort;                           // a wait that runs out ends this CTA only (about a second)
+    int launch_abort;                                   // a wait that runs out ends this CTA only (about a second)
     AbortBox box;
 };
-
-// What a CTA works on
-struct Job {
-    int n, w0, tiles;          // keys of the list, keys of the first tile, tiles
-    int sinks, first;          // list entry u is token u < sinks ? u : u - sinks + first of the table at `beg`
-    int64_t beg;
-    int hk;
-    int jb[2], je[2];          // tiles of each warpgroup (key_split: every second one from jb)
-};
-__device__ __forceinline__ int tile_base(const Job& job, int j) { return j ? job.w0 + (j - 1) * BN : 0; }
-__device__ __forceinline__ int tile_keys(const Job& job, int j) { return j ? BN : job.w0; }
-__device__ __forceinline__ int tile_of(const Job& job, int u) { return u < job.w0 ? 0 : (u - job.w0) / BN + 1; }
-__device__ __forceinline__ void cut(Job& job, int n) {
-    job.n = n;
-    job.tiles = (n + BN - 1) / BN;
-    job.w0 = n - (job.tiles - 1) * BN;
+__device__ __forceinline__ int tile_base(int w0, int j) { return j ? w0 + (j - 1) * BN : 0; }
+__device__ __forceinline__ int tile_keys(int w0, int j) { return j ? BN : w0; }
+__device__ __forceinline__ int tile_of(const Item& it, int u) { return u < it.w0 ? 0 : (u - it.w0) / BN + 1; }
+__device__ __forceinline__ void cut(Item& it, int n) {
+    it.n = n;
+    it.tiles = (n + BN - 1) / BN;
+    it.w0 = n - (it.tiles - 1) * BN;
 }
+__device__ __forceinline__ bool active(const Item& it, int w) { return it.je[w] > it.jb[w]; }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void st_shared16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(src) : "memory");
+    return x;
+}
+
+// Item `id` of a window launch (false: it has no query rows)
+__device__ __forceinline__ bool window_item(const AttendParams& p, int64_t id, Item& it) {
+    const int64_t bb = id / p.units;
+    const int unit = (int)(id - bb * p.units), b = (int)(bb / p.blocks), blk = (int)(bb - (int64_t)b * p.blocks), G = p.H / p.Hkv;
+    const int64_t q_beg = b ? p.q_offsets[b - 1] : 0, q_end = p.q_offsets[b];
+    const int64_t kv_beg = b ? p.kv_offsets[b - 1] : 0, kv_end = p.kv_offsets[b];
+    if (q_beg < 0 || q_end < q_beg || q_end > p.n_q_tokens || kv_beg < 0 || kv_end > p.n_kv_tokens || kv_end - kv_beg < q_end - q_beg) {
+        if (p.err_flag) atomicOr(p.err_flag, ATTN_B200_FLAG_BAD_OFFSETS);
+        return false;
+    }
+    const int q_len = (int)(q_end - q_beg), kv_len = (int)(kv_end - kv_beg), shift = kv_len - q_len;
+    const int rows = p.head_pairs ? BM : 2 * BM, q0 = blk * rows;
+    if (q0 >= q_len) return false;
+    if (p.head_pairs) {
+        it.hk = unit / (G / 2);
+        it.head[0] = unit * 2;
+        it.head[1] = unit * 2 + 1;
+        it.row0[0] = it.row0[1] = q0;
+    } else {
+        it.hk = unit / G;
+        it.head[0] = it.head[1] = unit;
+        it.row0[0] = q0;
+        it.row0[1] = q0 + BM;
+    }
+    const int last = shift + min(q0 + rows, q_len) - 1;
+    const int64_t lo = (int64_t)shift + q0 - p.window + 1;
+    it.first = lo > 0 ? (int)lo : 0;
+    it.sinks = min(p.sinks, it.first);
+    it.beg = kv_beg;
+    cut(it, it.sinks + last - it.first + 1);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        it.jb[w] = it.je[w] = 0;
+        if (it.row0[w] >= q_len) continue;
+        const int hi_w = shift + min(it.row0[w] + BM, q_len) - 1 - it.first + it.sinks;
+        const int64_t lo_w = (int64_t)shift + it.row0[w] - p.window + 1 - it.first + it.sinks;
+        it.je[w] = tile_of(it, hi_w) + 1;
+        it.jb[w] = p.sinks > 0 || lo_w <= 0 ? 0 : tile_of(it, (int)lo_w);
+    }
+    it.n_rows = q_len;
+    it.shift = shift;
+    it.q_beg = q_beg;
+    return true;
+}
+
+// The one item of a prefix CTA: its share of the key tiles (the list's first tile is the short one) for a pair
+// of query tiles of a KV head
+__device__ __forceinline__ void prefix_item(const AttendParams& p, Item& it) {
+    const int G = p.H / p.Hkv, per = p.splits * p.Hkv;
+    const int group = blockIdx.x / per, rest = blockIdx.x - group * per;
+    it.hk = rest / p.splits;
+    const int split = rest - it.hk * p.splits;
+    const int tiles = (p.n_prefix + BN - 1) / BN, short_keys = p.n_prefix - (tiles - 1) * BN;
+    const int a = (int)((int64_t)tiles * split / p.splits), e = (int)((int64_t)tiles * (split + 1) / p.splits);
+    const int u0 = a ? short_keys + (a - 1) * BN : 0, u1 = e ? short_keys + (e - 1) * BN : 0;
+    it.beg = u0;
+    it.sinks = it.first = 0;
+    cut(it, u1 - u0);
+    it.n_rows = p.B * G;
+    it.row0[0] = group * (p.key_split ? BM : 2 * BM);
+    it.row0[1] = it.row0[0] + (p.key_split ? 0 : BM);
+    it.head[0] = it.head[1] = 0;
+    it.jb[0] = 0;
+    it.jb[1] = p.key_split ? 1 : 0;
+    it.je[0] = it.tiles;
+    it.je[1] = it.row0[1] < it.n_rows ? it.tiles : 0;
+    it.shift = 0;
+    it.q_beg = 0;
+    it.part = split * (p.key_split ? 2 : 1);
+}
 
 // One softmax thread = one query row: walks `count` tiles from `j0` in steps of `step`, leaves P in tensor memory
 // over S, keeps the reference maximum m and the denominator l.  Visible entries u of the list: u <= hi and
-// (u >= lo or u < ns).  Returns false when a wait ran out.
+// (u >= lo or u < ns).  `c0`: tiles this warpgroup has seen before (barrier phases), `g0`: tiles of the CTA
+// before this item.  Returns false when a wait ran out.
 template <typename MT, int HD, int kPolyOf8>
-__device__ __forceinline__ bool softmax_rows(Smem<HD>& sm, int w, uint32_t s_addr, uint32_t o_addr, const Job& job, int j0, int step,
-                                             int count, int hi, int lo, int ns, float scale, float& m_ref, float& l) {
+__device__ __forceinline__ bool softmax_rows(Smem<HD>& sm, int w, uint32_t s_addr, uint32_t o_addr, int w0, int j0, int step,
+                                             int count, int c0, int g0, int hi, int lo, int ns, float scale, float& m_ref, float& l) {
     AbortBox* const wc = &sm.box;
     constexpr float kLazy = 8.f;          // P <= 2^8: O is rescaled rarely
     m_ref = -INFINITY;
@@ -94,7 +184,7 @@ __device__ __forceinline__ bool softmax_rows(Smem<HD>& sm, int w, uint32_t s_add
                 // a row that has seen nothing yet keeps its zeros (-inf - -inf is not a number)
                 const float alpha = m_ref == m_new ? 1.f : fast_exp2(m_ref - m_new);
                 l *= alpha;
-                if (!mbar_wait(&sm.o_full[w], (i - 1) & 1, wc)) return false;
+                if (!mbar_wait(&sm.o_full[w], (c0 + i - 1) & 1, wc)) return false;
                 tc_fence_after();
 #pragma unroll
                 for (int c = 0; c < HD / 32; ++c) {
@@ -111,28 +201,17 @@ __device__ __forceinline__ bool softmax_rows(Smem<HD>& sm, int w, uint32_t s_add
         return true;
     };
     for (int i = 0; i < count; ++i) {
-        const int j = j0 + i * step, base = tile_base(job, j), keys = tile_keys(job, j);
-        if (!mbar_wait(&sm.s_full[w], i & 1, wc)) return false;
+        const int j = j0 + i * step, base = tile_base(w0, j), keys = tile_keys(w0, j);
+        if (!mbar_wait(&sm.s_full[w], (c0 + i) & 1, wc)) return false;
         tc_fence_after();
         const bool any_bad = *(volatile int*)&sm.any_bad;
+        const unsigned char* const bad = sm.bad[(g0 + j) & 3];
         const int h = min(hi - base, keys - 1), lw = lo - base, s = ns - base;     // in columns of this tile
-        const bool masked = any_bad || h < BN - 1 || (lw > 0 && s < BN);
-        auto hidden = [&](int c) { return c > h || (c < lw && c >= s) || (any_bad && sm.bad[j & 3][c & (BN - 1)]); };
-        if (keys > 96) {
+        if (keys == BN && !__any_sync(0xffffffffu, any_bad || h < BN - 1 || (lw > 0 && s < BN))) {
             float sv[BN];
 #pragma unroll
             for (int c = 0; c < 4; ++c) tmem_ld32_nowait(s_addr + c * 32, sv + c * 32);
             tmem_ld_wait();
-            if (masked) {
-                if (any_bad) {
-#pragma unroll
-                    for (int c = 0; c < BN; ++c)
-                        if (sm.bad[j & 3][c]) sv[c] = -INFINITY;
-                }
-#pragma unroll
-                for (int c = 0; c < BN; ++c)
-                    if (c > h || (c < lw && c >= s)) sv[c] = -INFINITY;
-            }
             float mx8[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) mx8[e] = fmaxf(sv[e], sv[8 + e]);
@@ -174,133 +253,119 @@ __device__ __forceinline__ bool softmax_rows(Smem<HD>& sm, int w, uint32_t s_add
             }
             l += (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
         } else {
-            // a short first tile: 32 columns at a time, as many as it has
-            const int chunks = (keys + 31) / 32;
-            float mx = -INFINITY;
-            for (int c = 0; c < chunks; ++c) {
-                float sv[32];
-                tmem_ld32(s_addr + c * 32, sv);
+            // A tile at an end of a window, a short first tile, or missing rows: 32 columns at a time, read from tensor
+            // memory for the maximum and again for P.  Chunks that no row of the warp sees (half of the triangles at
+            // both ends) are neither read nor exponentiated, chunks that all rows see are not masked.
+            const int chunks = keys > 96 ? 4 : (keys + 31) / 32;
+            const int h_max = __reduce_max_sync(0xffffffffu, h), h_min = __reduce_min_sync(0xffffffffu, h);
+            const int lw_max = __reduce_max_sync(0xffffffffu, lw), lw_min = __reduce_min_sync(0xffffffffu, lw);
+            auto dead = [&](int c) { return c > h_max || (c + 31 < lw_min && c >= s); };
+            auto whole = [&](int c) { return !any_bad && c + 31 <= h_min && (c >= lw_max || c + 31 < s); };
+            // this row's visible columns of chunk c as bits
+            auto bits = [&](int c) -> uint32_t {
+                auto below = [&](int x) { return x <= c ? 0u : x >= c + 32 ? 0xffffffffu : (1u << (x - c)) - 1u; };     // columns < x
+                uint32_t m = below(h + 1) & (~below(lw) | below(s));
+                if (any_bad) {
+                    const uint32_t* b4 = reinterpret_cast<const uint32_t*>(bad + c);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) mx = fmaxf(mx, masked && hidden(c * 32 + e) ? -INFINITY : sv[e]);
+                    for (int e = 0; e < 8; ++e) m &= ~(((b4[e] & 1u) | (b4[e] >> 7 & 2u) | (b4[e] >> 14 & 4u) | (b4[e] >> 21 & 8u)) << (4 * e));
+                }
+                return m;
+            };
+            float mx = -INFINITY;
+            for (int c = 0; c < chunks * 32; c += 32) {
+                if (dead(c)) continue;
+                float sv[32];
+                tmem_ld32(s_addr + c, sv);
+                if (!whole(c)) {
+                    const uint32_t m = bits(c);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) sv[e] = m >> e & 1u ? sv[e] : -INFINITY;
+                }
+                float a = fmaxf(sv[0], sv[1]), b = fmaxf(sv[2], sv[3]);
+#pragma unroll
+                for (int e = 4; e < 32; e += 4) {
+                    a = max3(a, sv[e], sv[e + 1]);
+                    b = max3(b, sv[e + 2], sv[e + 3]);
+                }
+                mx = max3(mx, a, b);
             }
             if (!advance(i, mx)) return false;
             const float nm = m_ref > -INFINITY ? -m_ref : 0.f;
-            for (int c = 0; c < chunks; ++c) {       // P of chunk c lands on columns 16 c .., already read
-                float sv[32];
+            float l4[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int c = 0; c < chunks * 32; c += 32) {       // P of a chunk lands on columns c / 2 .., already read
                 uint32_t pk[16];
-                tmem_ld32(s_addr + c * 32, sv);
+                if (dead(c)) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const float p0 = masked && hidden(c * 32 + e) ? 0.f : fast_exp2(fmaf(sv[e], scale, nm));
-                    const float p1 = masked && hidden(c * 32 + e + 1) ? 0.f : fast_exp2(fmaf(sv[e + 1], scale, nm));
-                    l += p0 + p1;
-                    pk[e >> 1] = pack2<MT>(p0, p1);
+                    for (int e = 0; e < 16; ++e) pk[e] = 0u;
+                } else {
+                    float sv[32];
+                    tmem_ld32(s_addr + c, sv);
+                    const uint32_t m = whole(c) ? 0xffffffffu : bits(c);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        float x[4];
+                        fma2(x[0], x[1], sv[e], sv[e + 1], scale, scale, nm, nm);
+                        fma2(x[2], x[3], sv[e + 2], sv[e + 3], scale, scale, nm, nm);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            x[k] = m >> (e + k) & 1u ? fast_exp2(x[k]) : 0.f;
+                            l4[k] += x[k];
+                        }
+                        pk[e >> 1] = pack2<MT>(x[0], x[1]);
+                        pk[(e >> 1) + 1] = pack2<MT>(x[2], x[3]);
+                    }
                 }
                 asm volatile(
                     "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                    ::"r"(s_addr + c * 16), "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]), "r"(pk[4]), "r"(pk[5]), "r"(pk[6]),
+                    ::"r"(s_addr + (c >> 1)), "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]), "r"(pk[4]), "r"(pk[5]), "r"(pk[6]),
                       "r"(pk[7]), "r"(pk[8]), "r"(pk[9]), "r"(pk[10]), "r"(pk[11]), "r"(pk[12]), "r"(pk[13]), "r"(pk[14]),
                       "r"(pk[15]) : "memory");
-                tmem_st_wait();
+                if (c == 32 || (chunks == 1 && c == 0)) {      // the first 64 keys (of a short tile the MMA thread wants all)
+                    tmem_st_wait();
+                    tc_fence_before();
+                    mbar_arrive(&sm.p_half[w]);
+                }
             }
-            mbar_arrive(&sm.p_half[w]);
+            l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
         }
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&sm.p_full[w]);
     }
-    if (count > 0) {
-        if (!mbar_wait(&sm.o_full[w], (count - 1) & 1, wc)) return false;
-        tc_fence_after();
-    }
+    if (!mbar_wait(&sm.o_full[w], (c0 + count - 1) & 1, wc)) return false;
+    tc_fence_after();
     return true;
 }
 
-template <typename T, int HD, bool kPrefix, bool E4>
+// Roles.  Warps 0-3 and 4-7 softmax, 8 item list, 9 MMA thread, 10 and 11 query tiles, 12-13 K, 14-15 V.  A window
+// launch is persistent: one CTA per SM takes every gridDim.x-th item, and the item list, the query tiles and the K/V
+// rings run ahead of the softmax, so that the set-up of an item hides under the one before it.  A prefix CTA has
+// one item.
+enum Mode { kWindow, kPrefixPair, kPrefixSplit };      // kPrefixSplit: AttendParams::key_split
+template <typename T, int HD, int kMode, bool E4>
 __global__ void __launch_bounds__(kThreads, 1)
 attend_tc_kernel(const AttendParams p) {
+    constexpr bool kPrefix = kMode != kWindow, key_split = kMode == kPrefixSplit;
     using MT = typename std::conditional<E4, __half, T>::type;       // e4m3 rows are multiplied as fp16
+    using R = Regs<E4>;
     constexpr int kTileBytes = Smem<HD>::kTile;
-    constexpr int CPR = HD / 8, RPP = 64 / CPR, PASSES = BN / RPP;   // 16-byte chunks of a row; rows per pass of 64 threads
+    constexpr int QC = HD / 8;                                       // 16-byte chunks of a query row
     extern __shared__ unsigned char smem_raw[];
     Smem<HD>& sm = *reinterpret_cast<Smem<HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     AbortBox* const wc = &sm.box;
     const int G = p.H / p.Hkv;
 
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-    Job job;
-    int head[2] = {0, 0}, row0[2] = {0, 0};      // window: head and first query row (in the chunk) of each tile
-    int q_len = 0, shift = 0, t_first = 0;
-    int64_t q_beg = 0;
-    if (kPrefix) {
-        job.hk = blockIdx.y;
-        const int tiles = (p.n_prefix + BN - 1) / BN;
-        // this CTA's share of the key tiles; the list's first tile is the short one
-        const int a = (int)((int64_t)tiles * blockIdx.x / p.splits), e = (int)((int64_t)tiles * (blockIdx.x + 1) / p.splits);
-        const int short_keys = p.n_prefix - (tiles - 1) * BN;
-        const int u0 = a ? short_keys + (a - 1) * BN : 0, u1 = e ? short_keys + (e - 1) * BN : 0;
-        job.beg = u0;
-        job.sinks = job.first = 0;
-        cut(job, u1 - u0);
-        job.jb[0] = 0;
-        job.jb[1] = p.key_split ? 1 : 0;
-        job.je[0] = job.je[1] = job.tiles;
-        row0[0] = blockIdx.z * (p.key_split ? BM : 2 * BM);
-        row0[1] = row0[0] + (p.key_split ? 0 : BM);
-        if (row0[1] >= p.B * G) job.je[1] = 0;
-    } else {
-        const int b = blockIdx.z;
-        q_beg = b ? p.q_offsets[b - 1] : 0;
-        const int64_t q_end = p.q_offsets[b], kv_beg = b ? p.kv_offsets[b - 1] : 0, kv_end = p.kv_offsets[b];
-        if (q_beg < 0 || q_end < q_beg || q_end > p.n_q_tokens || kv_beg < 0 || kv_end > p.n_kv_tokens || kv_end - kv_beg < q_end - q_beg) {
-            if (p.err_flag && threadIdx.x == 0) atomicOr(p.err_flag, ATTN_B200_FLAG_BAD_OFFSETS);
-            return;
-        }
-        q_len = (int)(q_end - q_beg);
-        const int kv_len = (int)(kv_end - kv_beg);
-        shift = kv_len - q_len;
-        const int q0 = blockIdx.x * (p.head_pairs ? BM : 2 * BM);
-        if (q0 >= q_len) return;
-        if (p.head_pairs) {
-            const int per = G / 2;
-            job.hk = blockIdx.y / per;
-            head[0] = job.hk * G + (blockIdx.y - job.hk * per) * 2;
-            head[1] = head[0] + 1;
-            row0[0] = row0[1] = q0;
-        } else {
-            head[0] = head[1] = blockIdx.y;
-            job.hk = blockIdx.y / G;
-            row0[0] = q0;
-            row0[1] = q0 + BM;
-        }
-        const int rows = p.head_pairs ? BM : 2 * BM;
-        const int last = shift + min(q0 + rows, q_len) - 1;
-        const int64_t lo = (int64_t)shift + q0 - p.window + 1;
-        t_first = lo > 0 ? (int)lo : 0;
-        job.beg = kv_beg;
-        job.first = t_first;
-        job.sinks = min(p.sinks, t_first);
-        cut(job, job.sinks + last - t_first + 1);
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            if (row0[w] >= q_len) {
-                job.jb[w] = job.je[w] = 0;
-                continue;
-            }
-            const int hi_w = shift + min(row0[w] + BM, q_len) - 1 - t_first + job.sinks;
-            const int64_t lo_w = (int64_t)shift + row0[w] - p.window + 1 - t_first + job.sinks;
-            job.je[w] = tile_of(job, hi_w) + 1;
-            job.jb[w] = p.sinks > 0 || lo_w <= 0 ? 0 : tile_of(job, (int)lo_w);
-        }
-    }
-    const bool key_split = kPrefix && p.key_split;
-
     if (threadIdx.x == 0) {
+        for (int i = 0; i < kItems; ++i) {
+            mbar_init(&sm.item_full[i], 1);
+            mbar_init(&sm.item_empty[i], 15);       // one lane of every warp but the list's own
+        }
         for (int w = 0; w < 2; ++w) {
-            mbar_init(&sm.q_full[w], 128);
+            mbar_init(&sm.q_full[w], kPrefix ? 128 : 32);
+            mbar_init(&sm.q_empty[w], 1);
+            mbar_init(&sm.o_free[w], 128);
             mbar_init(&sm.s_full[w], 1);
             mbar_init(&sm.p_half[w], 128);
             mbar_init(&sm.p_full[w], 128);
@@ -313,8 +378,8 @@ attend_tc_kernel(const AttendParams p) {
             mbar_init(&sm.v_empty[s], 1);
         }
         sm.any_bad = 0;
-        sm.box.abort = 0;
         sm.launch_abort = 0;
+        sm.box.abort = 0;
         sm.box.launch_abort = &sm.launch_abort;
         sm.box.err_flag = p.err_flag;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -327,302 +392,467 @@ attend_tc_kernel(const AttendParams p) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
+    // everything above is the CTA's own; from here on it reads what earlier kernels wrote
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // n-th item of this CTA: null when there are no more (or a wait ran out)
+    auto next_item = [&](int n) -> const Item* {
+        if (!mbar_wait(&sm.item_full[n % kItems], (n / kItems) & 1, wc)) return nullptr;
+        const Item* it = &sm.item[n % kItems];
+        return it->tiles ? it : nullptr;
+    };
+    auto done_with = [&](int n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.item_empty[n % kItems]);
+    };
+    // Query rows row, row + step, ... of warpgroup w's tile: `at` is the row's element offset in q (and in the
+    // window's output), -1 past the end
+    struct Rows {
+        int64_t at0;
+        int left, g, G, stride;
+        __device__ __forceinline__ int64_t at() const { return left > 0 ? at0 : -1; }
+        __device__ __forceinline__ void next(int step) {
+            left -= step;
+            if (kPrefix) {              // row b G + g: head g of sequence b
+                at0 += step * HD;
+                for (g += step; g >= G; g -= G) at0 += stride;
+            } else {
+                at0 += (int64_t)step * stride;
+            }
+        }
+    };
+    auto rows_from = [&](const Item& it, int w, int row) -> Rows {
+        if (kPrefix) {
+            const int b = row / G, g = row - b * G;
+            return Rows{((int64_t)b * p.H + it.hk * G + g) * HD, it.n_rows - row, g, G, (p.H - G) * HD};
+        }
+        return Rows{((it.q_beg + row) * p.H + it.head[w]) * HD, it.n_rows - row, 0, 1, p.H * HD};
+    };
+    // A warp copies query rows r0 .. r0 + n - 1 of a tile into its swizzled place, whole rows at a time
+    auto load_q = [&](const Item& it, int w, int r0, int n) {
+        constexpr int kAtOnce = 32 / QC;
+        const int cc = lane % QC, rr = lane / QC;
+        const uint32_t dst = smem_u32(sm.q[w]) + (cc >> 3) * kSub;
+        Rows rows = rows_from(it, w, it.row0[w] + r0 + rr);
+        if constexpr (!(E4 && std::is_same<T, __nv_bfloat16>::value)) {
+#pragma unroll 8
+            for (int i = 0; i < n; i += kAtOnce) {
+                const int r = r0 + i + rr;
+                const int64_t at = rows.at();
+                cp16(dst + r * 128 + (((cc & 7) ^ (r & 7)) << 4), (const T*)p.q + (at >= 0 ? at : 0) + cc * 8, at >= 0 ? 16 : 0);
+                rows.next(kAtOnce);
+            }
+            asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+        } else {
+            // bf16 queries over e4m3 rows are multiplied as fp16, after a power of two that brings the row to [1, 2):
+            // nothing overflows, and what is lost is below 2^-24 of its largest entry
+#pragma unroll 4
+            for (int i = 0; i < n; i += kAtOnce) {
+                const int r = r0 + i + rr;
+                const int64_t at = rows.at();
+                const uint4 x = at >= 0 ? *reinterpret_cast<const uint4*>((const T*)p.q + at + cc * 8) : make_uint4(0, 0, 0, 0);
+                rows.next(kAtOnce);
+                const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
+                float f[8], top = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    unpack2(wd[e], T(), f[2 * e], f[2 * e + 1]);
+                    top = fmaxf(top, fmaxf(fabsf(f[2 * e]), fabsf(f[2 * e + 1])));
+                }
+                top = group_max<QC>(top);
+                int ex = 0;
+                if (top > 1e-30f && top < 1e30f) ex = ((__float_as_int(top) >> 23) & 255) - 127;
+                const float mul = __int_as_float((127 - ex) << 23);
+                if (cc == 0) sm.row_exp[w][r] = (signed char)ex;
+                st_shared16(dst + r * 128 + (((cc & 7) ^ (r & 7)) << 4), pack2<__half>(f[0] * mul, f[1] * mul), pack2<__half>(f[2] * mul, f[3] * mul),
+                            pack2<__half>(f[4] * mul, f[5] * mul), pack2<__half>(f[6] * mul, f[7] * mul));
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&sm.q_full[w]);
+    };
 
     if (warp >= 12) {
         // ------------------------------------------------------------------ gather: 64 threads K, 64 threads V
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<E4>::kGather));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::kGather));
+        constexpr int kRow = E4 ? HD : 2 * HD;                              // bytes of a head's row in the pool
+        constexpr int CPR = kRow / 16, RPP = 64 / CPR, PASSES = BN / RPP;   // chunks of a row; rows per pass of 64 threads
         const int tid = threadIdx.x - 384, t64 = tid & 63;
         const bool v_stream = tid >= 64;
         const int c = t64 % CPR, rsub = t64 / CPR;
         unsigned long long* full = v_stream ? sm.v_full : sm.k_full;
         unsigned long long* empty = v_stream ? sm.v_empty : sm.k_empty;
         unsigned char (*stage)[kTileBytes] = v_stream ? sm.v : sm.k;
-        // The CPR threads of a row group need the same PASSES slots: thread c fetches and checks those of
-        // passes c and c + CPR, the copies take them by shuffle.
-        // The slots of the next tile are fetched ahead of the wait for its stage.
-        int ahead[2];
-        auto fetch = [&](int j) {
+        const uint32_t raw = smem_u32(sm.extra[v_stream]) + t64 * 16;       // e4m3: this thread's chunk of pass 0
+        const int64_t row_bytes = (int64_t)p.Hkv * kRow;
+        int g = 0;                                                          // tiles of earlier items
+        for (int n = 0;; ++n) {
+            const Item* const ip = next_item(n);
+            if (__any_sync(0xffffffffu, !ip)) break;
+            const Item& it = *ip;
+            const int w0 = it.w0, tiles = it.tiles, sinks = it.sinks, skip = it.first - it.sinks;
+            const int32_t* const table = p.table + it.beg;
+            const char* const base = (const char*)(v_stream ? p.v_cache : p.k_cache) + (int64_t)it.hk * kRow + c * 16;
+            // The CPR threads of a row group need the same PASSES slots: thread c fetches and checks those of
+            // passes c and c + CPR (one tile ahead), the copies take them by shuffle.
+            int ahead[2];
+            auto fetch = [&](int j) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = (c + CPR * i) * RPP + rsub, u = tile_base(job, j) + r;
-                const int t = u < job.sinks ? u : u - job.sinks + job.first;
-                ahead[i] = j < job.tiles && r < tile_keys(job, j) ? __ldg(p.table + job.beg + t) : -1;
-            }
-        };
-        fetch(0);
-        bool ok = true;
-        for (int j = 0; j < job.tiles; ++j) {
-            const int s = j % kStages;
-            int sl[2] = {ahead[0], ahead[1]};
-            fetch(j + 1);
-            if (j >= kStages) ok = mbar_wait(&empty[s], ((j - kStages) / kStages) & 1, wc);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = (c + CPR * i) * RPP + rsub;
-                if (sl[i] < 0 || sl[i] >= p.n_slots) {
-                    bad |= r < tile_keys(job, j);
-                    sl[i] = -1;
+                for (int i = 0; i < 2; ++i) {
+                    const int r = (c + CPR * i) * RPP + rsub, u = tile_base(w0, j) + r;
+                    ahead[i] = j < tiles && r < tile_keys(w0, j) ? __ldg(table + (u < sinks ? u : u + skip)) : -1;
                 }
-                // bad[j & 3]: written before the tile is published and read until its P is there, which the
-                // products of tile j + 2 wait for; those precede the release that lets tile j + 4 in
-                if (!v_stream) sm.bad[j & 3][r] = sl[i] < 0;
-            }
-            if (bad) {
-                if (!v_stream) sm.any_bad = 1;
-                if (p.err_flag) atomicOr(p.err_flag, ATTN_B200_FLAG_BAD_SLOT);
-            }
-            if constexpr (!E4) {
-                const uint32_t sbase = smem_u32(stage[s]) + (c >> 3) * kSub;
-                const char* base = (const char*)(v_stream ? p.v_cache : p.k_cache) + ((int64_t)job.hk * HD + c * 8) * 2;
-                const int64_t row_bytes = (int64_t)p.Hkv * HD * 2;
+            };
+            // destination of row q RPP + rsub, chunk c: the row's low three bits are those of q RPP + rsub, so
+            // there are at most two swizzle terms per thread and everything else is a compile-time offset
+            const uint32_t swz0 = rsub * 128 + ((((uint32_t)c & 7) ^ (uint32_t)(rsub & 7)) << 4);
+            const uint32_t swz1 = rsub * 128 + ((((uint32_t)c & 7) ^ (uint32_t)((RPP + rsub) & 7)) << 4);
+            auto copy = [&](uint32_t dst, const int (&sl)[2]) {
+                const uint32_t d0 = dst + swz0, d1 = dst + swz1;
 #pragma unroll
                 for (int q = 0; q < PASSES; ++q) {
                     const int v = __shfl_sync(0xffffffffu, sl[q / CPR], q % CPR, CPR);
-                    const int r = q * RPP + rsub;
-                    cp16(sbase + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + (int64_t)(v >= 0 ? v : 0) * row_bytes, v >= 0 ? 16 : 0);
+                    cp16(E4 ? dst + q * 1024 : ((q & 1) ? d1 : d0) + q * (RPP * 128), base + (int64_t)(v >= 0 ? v : 0) * row_bytes, v >= 0 ? 16 : 0);
                 }
-                asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-            } else {
-                // 8-byte pieces (8 codes -> 16 bytes of fp16), kBatch rows in flight
-                constexpr int kBatch = 16;
-                const uint32_t sbase = smem_u32(stage[s]) + (c >> 3) * kSub;
-                const char* base = (const char*)(v_stream ? p.v_cache : p.k_cache) + (int64_t)job.hk * HD + c * 8;
-                const int64_t row_bytes = (int64_t)p.Hkv * HD;
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            auto checked = [&](int (&sl)[2]) {       // slots outside the pools become -1
 #pragma unroll
-                for (int q0 = 0; q0 < PASSES; q0 += kBatch) {
-                    uint2 x[kBatch];
+                for (int i = 0; i < 2; ++i) sl[i] = ahead[i] >= 0 && ahead[i] < p.n_slots ? ahead[i] : -1;
+            };
+            // bad[tile & 3]: written before the tile is published and read until its P is there, which the MMA thread
+            // waits for before it issues anything of two tiles later and so before the release that lets the
+            // tile after next but one in
+            auto mark = [&](int j, const int (&sl)[2]) {
+                bool bad = false;
 #pragma unroll
-                    for (int q = 0; q < kBatch; ++q) {
-                        const int v = __shfl_sync(0xffffffffu, sl[(q0 + q) / CPR], (q0 + q) % CPR, CPR);
-                        x[q] = make_uint2(0, 0);
-                        if (v >= 0) x[q] = __ldg(reinterpret_cast<const uint2*>(base + (int64_t)v * row_bytes));
+                for (int i = 0; i < 2; ++i) {
+                    const int r = (c + CPR * i) * RPP + rsub;
+                    bad |= r < tile_keys(w0, j) && sl[i] < 0;
+                    if (!v_stream) sm.bad[(g + j) & 3][r] = sl[i] < 0;
+                }
+                if (bad) {
+                    if (!v_stream) sm.any_bad = 1;
+                    if (p.err_flag) atomicOr(p.err_flag, ATTN_B200_FLAG_BAD_SLOT);
+                }
+            };
+            fetch(0);
+            int sl[2];
+            checked(sl);
+            if (E4) copy(raw, sl);        // the raw rows of a tile travel while the tile before it is still in use
+            bool ok = true;
+            for (int j = 0; j < tiles; ++j) {
+                const int t = g + j, s = t % kStages;
+                fetch(j + 1);
+                if (t >= kStages) ok = mbar_wait(&empty[s], ((t - kStages) / kStages) & 1, wc);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                mark(j, sl);
+                if constexpr (!E4) {
+                    copy(smem_u32(stage[s]) + (c >> 3) * kSub, sl);
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                } else {
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    // 16 codes -> chunks 2 c and 2 c + 1 of the row in fp16; a thread reads what it copied itself
+                    const uint32_t dst = smem_u32(stage[s]) + (c >> 2) * kSub;
+#pragma unroll 4
+                    for (int q = 0; q < PASSES; ++q) {
+                        const int r = q * RPP + rsub;
+                        const uint4 x = ld_shared16(raw + q * 1024);
+                        __half2 h[8];
+                        e4m3x4_to_half2x2(x.x, h[0], h[1]);
+                        e4m3x4_to_half2x2(x.y, h[2], h[3]);
+                        e4m3x4_to_half2x2(x.z, h[4], h[5]);
+                        e4m3x4_to_half2x2(x.w, h[6], h[7]);
+                        const uint32_t* u = reinterpret_cast<const uint32_t*>(h);
+                        const uint32_t at = dst + r * 128;
+                        st_shared16(at + ((((2 * c) & 7) ^ (r & 7)) << 4), u[0], u[1], u[2], u[3]);
+                        st_shared16(at + ((((2 * c + 1) & 7) ^ (r & 7)) << 4), u[4], u[5], u[6], u[7]);
                     }
-#pragma unroll
-                    for (int q = 0; q < kBatch; ++q) {
-                        const int r = (q0 + q) * RPP + rsub;
-                        __half2 h0, h1, h2, h3;
-                        e4m3x4_to_half2x2(x[q].x, h0, h1);
-                        e4m3x4_to_half2x2(x[q].y, h2, h3);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sbase + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
-                                     "r"(*reinterpret_cast<uint32_t*>(&h0)), "r"(*reinterpret_cast<uint32_t*>(&h1)),
-                                     "r"(*reinterpret_cast<uint32_t*>(&h2)), "r"(*reinterpret_cast<uint32_t*>(&h3)) : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&full[s]);
+                checked(sl);
+                if (E4 && j + 1 < tiles) copy(raw, sl);
+            }
+            if (!__all_sync(0xffffffffu, ok)) break;
+            g += tiles;
+            done_with(n);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::kOther));
+        if (warp == 8) {
+            // -------------------------------------------------------------- item list
+            if (lane == 0) {
+                int64_t id = blockIdx.x;
+                for (int n = 0;; ++n) {
+                    if (n >= kItems && !mbar_wait(&sm.item_empty[n % kItems], (n / kItems - 1) & 1, wc)) break;
+                    Item& it = sm.item[n % kItems];
+                    it.tiles = 0;
+                    if (kPrefix) {
+                        if (n == 0) prefix_item(p, it);
+                    } else {
+                        bool found = false;
+                        for (; id < p.n_items && !found; id += gridDim.x) found = window_item(p, id, it);
+                        if (!found) it.tiles = 0;
                     }
+                    const bool end = it.tiles == 0;
+                    mbar_arrive(&sm.item_full[n % kItems]);
+                    if (end) break;
                 }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&full[s]);
-        }
-    } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<E4>::kOther));
-        if (warp == 9) {
+        } else if (warp == 9) {
             // -------------------------------------------------------------- MMA issuer
             constexpr uint32_t fmt = std::is_same<MT, __nv_bfloat16>::value ? 1u : 0u;
             constexpr uint32_t idesc0 = (1u << 4) | (fmt << 7) | (fmt << 10) | ((BM >> 4) << 24);
             constexpr uint32_t idesc_pv = idesc0 | (1u << 16) | ((HD >> 3) << 17);
             if (elect_one()) {
-                const uint64_t qd[2] = {smem_desc(smem_u32(sm.q[0]), 16, 1024), smem_desc(smem_u32(sm.q[key_split ? 0 : 1]), 16, 1024)};
-                const uint64_t kd[2] = {smem_desc(smem_u32(sm.k[0]), 16, 1024), smem_desc(smem_u32(sm.k[1]), 16, 1024)};
-                const uint64_t vd[2] = {smem_desc(smem_u32(sm.v[0]), kSub, 1024), smem_desc(smem_u32(sm.v[1]), kSub, 1024)};
-                // columns that a tile is multiplied in: whole, or its keys rounded up to 32
-                auto wide = [&](int j) { const int k = tile_keys(job, j); return k > 96 ? BN : (k + 31) / 32 * 32; };
-                auto issue_qk = [&](int w, int j) {
-                    const uint64_t a = qd[w], b2 = kd[j & 1];
-                    const uint32_t idesc = idesc0 | ((uint32_t)(wide(j) >> 3) << 17);
+                const uint64_t qd = smem_desc(smem_u32(sm.q[0]), 16, 1024), kd = smem_desc(smem_u32(sm.k[0]), 16, 1024);
+                const uint64_t vd = smem_desc(smem_u32(sm.v[0]), kSub, 1024);
+                constexpr uint64_t kTile16 = kTileBytes >> 4;
+                int g = 0;                       // tiles of earlier items
+                int done0 = 0, done1 = 0;        // tiles of each warpgroup whose P.V has been issued
+                int uses0 = 0, uses1 = 0;        // items in which it had work
+                // W: the warpgroup, a compile-time 0 or 1, so that all of this stays in registers
+                auto start_tile = [&](auto W, int t, int wide) -> bool {                  // Q.K of tile t (of the CTA)
+                    constexpr int w = decltype(W)::value;
+                    if (!mbar_wait_spin(&sm.k_full[t & 1], (t >> 1) & 1, wc)) return false;
+                    tc_fence_after();
+                    const uint64_t a = qd + (w ? (key_split ? 0 : kTile16) : 0), b2 = kd + (t & 1) * kTile16;
+                    const uint32_t idesc = idesc0 | ((uint32_t)(wide >> 3) << 17);
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk) {
                         const uint32_t off16 = ((kk >> 2) * kSub + (kk & 3) * 32) >> 4;
                         umma_f16(tmem + w * 128, a + off16, b2 + off16, idesc, kk > 0);
                     }
                     umma_commit(&sm.s_full[w]);
+                    return true;
                 };
-                auto pv_step = [&](int w, uint64_t v, int kk, bool first) {           // 16 keys
-                    umma_f16_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8, v + (uint64_t)(kk * (2048 >> 4)), idesc_pv, (!first || kk > 0) ? 1u : 0u);
-                };
-                int done[2] = {0, 0};            // tiles of each warpgroup whose P.V has been issued
-                bool ok = true;
-                auto finish_tile = [&](int w, int j) -> bool {        // P.V of tile j
-                    const int i = done[w];
-                    if (!mbar_wait_spin(&sm.p_half[w], i & 1, wc)) return false;
-                    if (!mbar_wait_spin(&sm.v_full[j & 1], (j >> 1) & 1, wc)) return false;
+                auto finish_tile = [&](auto W, int t, int wide, bool first) -> bool {     // P.V of tile t
+                    constexpr int w = decltype(W)::value;
+                    int& done = w ? done1 : done0;
+                    const uint32_t ph = done & 1;
+                    ++done;
+                    const uint64_t v = vd + (t & 1) * kTile16;
+                    const uint32_t d = tmem + 256 + w * 128, a = tmem + w * 128;
+                    if (first && (w ? uses1 : uses0) > 0 && !mbar_wait_spin(&sm.o_free[w], ((w ? uses1 : uses0) - 1) & 1, wc)) return false;
+                    if (!mbar_wait_spin(&sm.p_half[w], ph, wc)) return false;
+                    if (!mbar_wait_spin(&sm.v_full[t & 1], (t >> 1) & 1, wc)) return false;
                     tc_fence_after();
-                    const bool whole = wide(j) == BN;
-                    const uint64_t v = vd[j & 1];
-                    if (whole) {
+                    if (wide == BN) {
 #pragma unroll
-                        for (int kk = 0; kk < BN / 32; ++kk) pv_step(w, v, kk, i == 0);
-                    }
-                    if (!mbar_wait_spin(&sm.p_full[w], i & 1, wc)) return false;
-                    tc_fence_after();
-                    if (whole) {
+                        for (int kk = 0; kk < BN / 32; ++kk) umma_f16_ts(d, a + kk * 8, v + ((kk * 2048) >> 4), idesc_pv, (!first || kk > 0) ? 1u : 0u);
+                        if (!mbar_wait_spin(&sm.p_full[w], ph, wc)) return false;
+                        tc_fence_after();
 #pragma unroll
-                        for (int kk = BN / 32; kk < BN / 16; ++kk) pv_step(w, v, kk, false);
+                        for (int kk = BN / 32; kk < BN / 16; ++kk) umma_f16_ts(d, a + kk * 8, v + ((kk * 2048) >> 4), idesc_pv, 1u);
                     } else {
+                        if (!mbar_wait_spin(&sm.p_full[w], ph, wc)) return false;
+                        tc_fence_after();
 #pragma unroll 1
-                        for (int kk = 0; kk < wide(j) / 16; ++kk) pv_step(w, v, kk, i == 0);
+                        for (int kk = 0; kk < wide / 16; ++kk)
+                            umma_f16_ts(d, a + kk * 8, v + (uint64_t)(kk * (2048 >> 4)), idesc_pv, (!first || kk > 0) ? 1u : 0u);
                     }
                     umma_commit(&sm.o_full[w]);
-                    done[w] = i + 1;
                     return true;
                 };
-                auto start_tile = [&](int w, int j) -> bool {         // Q.K of tile j
-                    if (!mbar_wait_spin(&sm.k_full[j & 1], (j >> 1) & 1, wc)) return false;
-                    tc_fence_after();
-                    issue_qk(w, j);
-                    return true;
-                };
-                ok = mbar_wait_spin(&sm.q_full[0], 0, wc);
-                if (ok && !key_split) ok = mbar_wait_spin(&sm.q_full[1], 0, wc);
-                if (key_split) {
-                    for (int j = 0; ok && j < 2 && j < job.tiles; ++j) {
-                        ok = start_tile(j, j);
-                        umma_commit(&sm.k_empty[j & 1]);
-                    }
-                    for (int j = 0; ok && j < job.tiles; ++j) {
-                        if (!(ok = finish_tile(j & 1, j))) break;
-                        umma_commit(&sm.v_empty[j & 1]);
-                        if (j + 2 < job.tiles) {
-                            if (!(ok = start_tile(j & 1, j + 2))) break;
-                            umma_commit(&sm.k_empty[j & 1]);
+                const std::integral_constant<int, 0> W0{};
+                const std::integral_constant<int, 1> W1{};
+                for (int n = 0;; ++n) {
+                    const Item* const ip = next_item(n);
+                    if (!ip) break;
+                    const int tiles = ip->tiles, jb0 = ip->jb[0], jb1 = ip->jb[1], je0 = ip->je[0], je1 = ip->je[1];
+                    // columns that a tile is multiplied in: whole, or its keys rounded up to 32
+                    const int wide0 = ip->w0 > 96 ? BN : (ip->w0 + 31) / 32 * 32;
+                    auto wide = [&](int j) { return j ? BN : wide0; };
+                    bool ok = mbar_wait_spin(&sm.q_full[0], uses0 & 1, wc);        // the first query tile always has rows
+                    if (key_split) {
+                        if (ok) ok = start_tile(W0, 0, wide0);
+                        umma_commit(&sm.k_empty[0]);
+                        if (ok && tiles > 1) {
+                            ok = start_tile(W1, 1, BN);
+                            umma_commit(&sm.k_empty[1]);
+                        }
+                        for (int j = 0; ok && j < tiles; j += 2) {
+                            if (!(ok = finish_tile(W0, j, wide(j), j == 0))) break;
+                            umma_commit(&sm.v_empty[0]);
+                            if (j + 2 < tiles) {
+                                if (!(ok = start_tile(W0, j + 2, BN))) break;
+                                umma_commit(&sm.k_empty[0]);
+                            }
+                            if (j + 1 == tiles) break;
+                            if (!(ok = finish_tile(W1, j + 1, BN, j == 0))) break;
+                            umma_commit(&sm.v_empty[1]);
+                            if (j + 3 < tiles) {
+                                if (!(ok = start_tile(W1, j + 3, BN))) break;
+                                umma_commit(&sm.k_empty[1]);
+                            }
+                        }
+                    } else {
+                        if (ok && je1 > jb1) ok = mbar_wait_spin(&sm.q_full[1], uses1 & 1, wc);
+                        // every tile is some warpgroup's: the list is the union of two overlapping stretches
+                        if (ok && jb0 == 0) ok = start_tile(W0, g, wide0);
+                        if (ok && je0 == 1) umma_commit(&sm.q_empty[0]);
+                        if (ok && jb1 == 0 && je1 > 0) {
+                            ok = start_tile(W1, g, wide0);
+                            if (je1 == 1) umma_commit(&sm.q_empty[1]);
+                        }
+                        umma_commit(&sm.k_empty[g & 1]);
+                        for (int j = 0; ok && j < tiles; ++j) {
+                            const int t = g + j;
+                            if (j >= jb0 && j < je0 && !(ok = finish_tile(W0, t, wide(j), j == jb0))) break;
+                            if (j + 1 >= jb0 && j + 1 < je0) {
+                                if (!(ok = start_tile(W0, t + 1, BN))) break;
+                                if (j + 2 == je0) umma_commit(&sm.q_empty[0]);
+                            }
+                            if (j >= jb1 && j < je1 && !(ok = finish_tile(W1, t, wide(j), j == jb1))) break;
+                            umma_commit(&sm.v_empty[t & 1]);
+                            if (j + 1 >= jb1 && j + 1 < je1) {
+                                if (!(ok = start_tile(W1, t + 1, BN))) break;
+                                if (j + 2 == je1) umma_commit(&sm.q_empty[1]);
+                            }
+                            if (j + 1 < tiles) umma_commit(&sm.k_empty[(t + 1) & 1]);
                         }
                     }
-                } else {
-                    // every tile is some warpgroup's: the list is the union of two overlapping stretches
-                    auto mine = [&](int w, int j) { return j >= job.jb[w] && j < job.je[w]; };
-                    for (int w = 0; w < 2 && ok; ++w)
-                        if (mine(w, 0)) ok = start_tile(w, 0);
-                    if (ok) umma_commit(&sm.k_empty[0]);
-                    for (int j = 0; ok && j < job.tiles; ++j) {
-                        for (int w = 0; w < 2 && ok; ++w) {
-                            if (mine(w, j)) ok = finish_tile(w, j);
-                            if (ok && w == 1) umma_commit(&sm.v_empty[j & 1]);
-                            if (ok && mine(w, j + 1)) ok = start_tile(w, j + 1);
-                        }
-                        if (ok && j + 1 < job.tiles) umma_commit(&sm.k_empty[(j + 1) & 1]);
-                    }
+                    if (!ok) break;
+                    uses0 += je0 > jb0;
+                    uses1 += je1 > jb1;
+                    g += tiles;
+                    mbar_arrive(&sm.item_empty[n % kItems]);
                 }
             }
             __syncwarp();
+        } else {
+            // -------------------------------------------------------------- window: query tile of warpgroup `w`
+            const int w = warp - 10;
+            int uses = 0;
+            for (int n = 0;; ++n) {
+                const Item* const ip = next_item(n);
+                if (__any_sync(0xffffffffu, !ip)) break;
+                const Item& it = *ip;
+                if (!kPrefix && active(it, w)) {
+                    const bool ok = uses == 0 || mbar_wait(&sm.q_empty[w], (uses - 1) & 1, wc);
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                    load_q(it, w, 0, BM);
+                    ++uses;
+                }
+                done_with(n);
+            }
         }
     } else {
         // ------------------------------------------------------------------ softmax warpgroups
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<E4>::kSoftmax));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R::kSoftmax));
         const int w = warp >> 2, r = threadIdx.x & 127;
-        const int n_rows = kPrefix ? p.B * G : q_len;
-        // element offset of row `row` of this warpgroup's tile in q (and in the window's output), or -1
-        auto row_at = [&](int row) -> int64_t {
-            if (row >= n_rows) return -1;
-            if (kPrefix) {
-                const int b = row / G;
-                return ((int64_t)b * p.H + job.hk * G + (row - b * G)) * HD;
-            }
-            return ((q_beg + row) * p.H + head[w]) * HD;
-        };
-        float scale = p.scale_log2;
-        if (kPrefix && E4) scale *= p.k_scale[job.hk];
-        if (!E4) {
-            if (w == 0 || !key_split) {
-                // a warp copies its own 32 rows, whole rows at a time, into the swizzled tile
-                constexpr int rows_at_once = 32 / CPR;
-                const int cc = lane % CPR, rr = lane / CPR;
-#pragma unroll 4
-                for (int i = 0; i < 32 / rows_at_once; ++i) {
-                    const int lr = (warp & 3) * 32 + i * rows_at_once + rr;
-                    const int64_t at = row_at(row0[w] + lr);
-                    cp16(smem_u32(sm.q[w]) + (cc >> 3) * kSub + lr * 128 + (((cc & 7) ^ (lr & 7)) << 4),
-                         (const T*)p.q + (at >= 0 ? at : 0) + cc * 8, at >= 0 ? 16 : 0);
-                }
-                asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-            }
-        } else {
-            // queries are multiplied as fp16: bf16 ones after a power of two that brings the row to [1, 2)
-            const int64_t at = row_at(row0[w] + r);
-            float mul = 1.f;
-            if (std::is_same<T, __nv_bfloat16>::value) {
-                float top = 0.f;
-                for (int d = 0; d < HD; d += 8) {
-                    const uint4 x = at >= 0 ? *reinterpret_cast<const uint4*>((const T*)p.q + at + d) : make_uint4(0, 0, 0, 0);
-                    const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float a, b;
-                        unpack2(wd[e], T(), a, b);
-                        top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
-                    }
-                }
-                if (top > 1e-30f && top < 1e30f) {
-                    const int ex = ((__float_as_int(top) >> 23) & 255) - 127;
-                    mul = __int_as_float((127 - ex) << 23);
-                    scale *= __int_as_float((127 + ex) << 23);
-                }
-            }
-            if (w == 0 || !key_split) {
-                for (int cc = 0; cc < CPR; ++cc) {
-                    uint4 x = at >= 0 ? *reinterpret_cast<const uint4*>((const T*)p.q + at + cc * 8) : make_uint4(0, 0, 0, 0);
-                    if (std::is_same<T, __nv_bfloat16>::value) {
-                        uint32_t wd[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float a, b;
-                            unpack2(wd[e], T(), a, b);
-                            wd[e] = pack2<__half>(a * mul, b * mul);
-                        }
-                        x = make_uint4(wd[0], wd[1], wd[2], wd[3]);
-                    }
-                    *reinterpret_cast<uint4*>(sm.q[w] + (cc >> 3) * kSub + r * 128 + (((cc & 7) ^ (r & 7)) << 4)) = x;
-                }
-            }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(&sm.q_full[w]);
-
         const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t s_addr = lane_base + w * 128, o_addr = lane_base + 256 + w * 128;
-        const int step = key_split ? 2 : 1;
-        const int count = job.je[w] > job.jb[w] ? (job.je[w] - job.jb[w] + step - 1) / step : 0;
-        const int row = row0[w] + r;
-        int hi = INT_MAX, lo = 0, ns = 0;
-        if (!kPrefix) {
-            hi = shift + row - t_first + job.sinks;
-            const int64_t lo64 = (int64_t)hi - p.window + 1;
-            lo = lo64 > 0 ? (int)lo64 : 0;
-            ns = p.sinks;
-        }
-        float m, l;
-        // e4m3 and fp16: every exponential on the special-function unit; bf16: two of eight as a cubic on the FMA pipe
-        const bool ok = softmax_rows<MT, HD, std::is_same<MT, __nv_bfloat16>::value ? 2 : 0>(sm, w, s_addr, o_addr, job, job.jb[w], step,
-                                                                                             count, hi, lo, ns, scale, m, l);
-        const int64_t at = row_at(row);
-        if (ok && kPrefix) {
-            const int b = row / G;
-            float* dst = p.parts + (((int64_t)(blockIdx.x * step + (key_split ? w : 0)) * p.B + b) * p.H + job.hk * G + (row - b * G)) * (HD + 2);
-            const float vs = E4 ? p.v_scale[job.hk] : 1.f;
-#pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-                float ov[32];
-                __syncwarp();
-                if (count > 0) tmem_ld32(o_addr + c * 32, ov);
-#pragma unroll
-                for (int e = 0; e < 32 && at >= 0; e += 2)
-                    *reinterpret_cast<float2*>(dst + c * 32 + e) =
-                        count > 0 ? make_float2(ov[e] * vs, ov[e + 1] * vs) : make_float2(0.f, 0.f);
+        constexpr int step = key_split ? 2 : 1;
+        int c0 = 0, g = 0;
+        for (int n = 0;; ++n) {
+            const Item* const ip = next_item(n);
+            if (__any_sync(0xffffffffu, !ip)) break;
+            const Item& it = *ip;
+            const int count = active(it, w) ? (it.je[w] - it.jb[w] + step - 1) / step : 0;
+            const int row = it.row0[w] + r;
+            int hi = INT_MAX, lo = 0, ns = 0;
+            if (!kPrefix) {
+                hi = it.shift + row - it.first + it.sinks;
+                const int64_t lo64 = (int64_t)hi - p.window + 1;
+                lo = lo64 > 0 ? (int)lo64 : 0;
+                ns = p.sinks;
             }
-            if (at >= 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(count > 0 ? m : -INFINITY, l);
-        } else if (ok && count > 0) {
-            // a row none of whose keys has a pool row is zero
-            const float inv = m > -INFINITY || l != l ? 1.f / l : 0.f;
-#pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-                float ov[32];
-                __syncwarp();
-                tmem_ld32(o_addr + c * 32, ov);
-                uint4* dst = reinterpret_cast<uint4*>((T*)p.out + (at >= 0 ? at : 0) + c * 32);
-#pragma unroll
-                for (int e = 0; e < 4 && at >= 0; ++e)
-                    dst[e] = make_uint4(pack2<T>(ov[8 * e] * inv, ov[8 * e + 1] * inv), pack2<T>(ov[8 * e + 2] * inv, ov[8 * e + 3] * inv),
-                                        pack2<T>(ov[8 * e + 4] * inv, ov[8 * e + 5] * inv), pack2<T>(ov[8 * e + 6] * inv, ov[8 * e + 7] * inv));
+            // a prefix CTA has one item, whose queries the softmax warps fetch themselves
+            if (kPrefix && count > 0 && !(key_split && w == 1)) load_q(it, w, (warp & 3) * 32, 32);
+            float scale = p.scale_log2, m = -INFINITY, l = 0.f;
+            if (kPrefix && E4) {
+                scale *= p.k_scale[it.hk];
+                if (std::is_same<T, __nv_bfloat16>::value && count > 0) {
+                    // the row's power of two is there when its first scores are
+                    if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[w], c0 & 1, wc))) break;
+                    scale *= __int_as_float((127 + sm.row_exp[key_split ? 0 : w][r]) << 23);
+                }
             }
+            // fp16: every exponential on the special-function unit; bf16: two of eight as a cubic on the FMA pipe
+            if (count > 0 && !__all_sync(0xffffffffu, softmax_rows<MT, HD, std::is_same<MT, __nv_bfloat16>::value ? 2 : 0>(
+                                                          sm, w, s_addr, o_addr, it.w0, it.jb[w], step, count, c0, g, hi, lo, ns, scale, m, l)))
+                break;
+            c0 += count;
+            g += it.tiles;
+            // The accumulator goes to registers, from there through shared memory (a warp its own rows, 16-byte
+            // chunks swizzled by the row) and leaves in whole rows: written straight from registers every
+            // store instruction touches 32 rows.
+            const int lr = lane, row_w = it.row0[w] + (warp & 3) * 32;       // this warp's first row
+            if (kPrefix) {
+                const float vs = E4 ? p.v_scale[it.hk] : 1.f;
+                const int64_t set = (int64_t)p.B * p.H, part = it.part + (key_split ? w : 0);
+                float2* const ml = reinterpret_cast<float2*>(p.parts + (int64_t)attend_prefix_parts(p) * set * HD);
+                const uint32_t buf = smem_u32(sm.q[w]) + (warp & 3) * (kTileBytes / 4);
+                constexpr int kCols = kTileBytes / BM / 4;                  // floats per row and pass
+#pragma unroll
+                for (int c = 0; c < HD; c += kCols) {
+                    const uint32_t mine = buf + lr * (kCols * 4);
+                    if (count > 0) {
+                        float ov[kCols];
+#pragma unroll
+                        for (int e = 0; e < kCols; e += 32) tmem_ld32(o_addr + c + e, ov + e);
+#pragma unroll
+                        for (int e = 0; e < kCols / 4; ++e)
+                            st_shared16(mine + ((e ^ (lr & (kCols / 4 - 1))) << 4), __float_as_uint(ov[4 * e] * vs), __float_as_uint(ov[4 * e + 1] * vs),
+                                        __float_as_uint(ov[4 * e + 2] * vs), __float_as_uint(ov[4 * e + 3] * vs));
+                    } else {
+                        for (int e = 0; e < kCols / 4; ++e) st_shared16(mine + (e << 4), 0, 0, 0, 0);
+                    }
+                    __syncwarp();
+                    constexpr int kLanes = kCols / 4, kRows = 32 / kLanes;   // lanes per row, rows per store
+                    Rows rows = rows_from(it, w, row_w + lane / kLanes);
+                    float* const dst = p.parts + part * set * HD + c + lane % kLanes * 4;
+#pragma unroll 8
+                    for (int i = 0; i < 32; i += kRows) {
+                        const int rr = i + lane / kLanes, cc = lane % kLanes;
+                        const uint4 x = ld_shared16(buf + rr * (kCols * 4) + ((cc ^ (rr & (kLanes - 1))) << 4));
+                        const int64_t at = rows.at();
+                        if (at >= 0) *reinterpret_cast<uint4*>(dst + at) = x;
+                        rows.next(kRows);
+                    }
+                    __syncwarp();
+                }
+                const int64_t at = rows_from(it, w, row).at();
+                if (at >= 0) ml[part * set + at / HD] = make_float2(count > 0 ? m : -INFINITY, l);
+            } else if (count > 0) {
+                float ov[HD];
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) tmem_ld32_nowait(o_addr + c * 32, ov + c * 32);
+                tmem_ld_wait();
+                tc_fence_before();
+                mbar_arrive(&sm.o_free[w]);         // the next item may overwrite the accumulator
+                // a row none of whose keys has a pool row is zero
+                const float inv = m > -INFINITY || l != l ? 1.f / l : 0.f;
+                constexpr int kPass = kTileBytes / 2 / BM / 2;              // columns per pass: half a row
+                const uint32_t buf = smem_u32(sm.extra[w]) + (warp & 3) * (kTileBytes / 8);
+#pragma unroll
+                for (int c = 0; c < HD; c += kPass) {
+#pragma unroll
+                    for (int e = 0; e < kPass / 8; ++e) {
+                        const float* o8 = ov + c + e * 8;
+                        st_shared16(buf + lr * (kPass * 2) + ((e ^ (lr & (kPass / 8 - 1))) << 4), pack2<T>(o8[0] * inv, o8[1] * inv),
+                                    pack2<T>(o8[2] * inv, o8[3] * inv), pack2<T>(o8[4] * inv, o8[5] * inv), pack2<T>(o8[6] * inv, o8[7] * inv));
+                    }
+                    __syncwarp();
+                    constexpr int kLanes = kPass / 8, kRows = 32 / kLanes;
+                    Rows rows = rows_from(it, w, row_w + lane / kLanes);
+                    T* const dst = (T*)p.out + c + lane % kLanes * 8;
+#pragma unroll
+                    for (int i = 0; i < 32; i += kRows) {
+                        const int rr = i + lane / kLanes, cc = lane % kLanes;
+                        const uint4 x = ld_shared16(buf + rr * (kPass * 2) + ((cc ^ (rr & (kLanes - 1))) << 4));
+                        const int64_t at = rows.at();
+                        if (at >= 0) *reinterpret_cast<uint4*>(dst + at) = x;
+                        rows.next(kRows);
+                    }
+                    __syncwarp();
+                }
+            }
+            done_with(n);
         }
     }
     tc_fence_before();
@@ -677,7 +907,9 @@ int launch_dependent(void (*kernel)(A...), dim3 grid, int threads, int smem, cud
     return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <typename T, int HD, bool kPrefix, bool E4>
+static_assert(sizeof(Smem<128>) + 1024 <= 227 * 1024, "shared memory");
+
+template <typename T, int HD, int kMode, bool E4>
 int launch(const AttendParams& p, dim3 grid, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
     const int smem = (int)sizeof(Smem<HD>) + 1024;
@@ -686,11 +918,11 @@ int launch(const AttendParams& p, dim3 grid, cudaStream_t st) {
     if (e != cudaSuccess) return (int)e;
     if (dev >= 64) return ATTN_B200_ETOOLARGE;
     if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
-        if ((e = cudaFuncSetAttribute(attend_tc_kernel<T, HD, kPrefix, E4>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess)
+        if ((e = cudaFuncSetAttribute(attend_tc_kernel<T, HD, kMode, E4>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess)
             return (int)e;
         ready.fetch_or(1ull << dev, std::memory_order_release);
     }
-    return launch_dependent(attend_tc_kernel<T, HD, kPrefix, E4>, grid, kThreads, smem, st, p);
+    return launch_dependent(attend_tc_kernel<T, HD, kMode, E4>, grid, kThreads, smem, st, p);
 }
 
 }  // namespace
@@ -711,10 +943,13 @@ int attend_window_launch(AttendParams p, int max_q_len, int D, int dtype, cudaSt
         if (rc) return rc;
     }
     if (blocks == 0 || p.B == 0) return 0;
-    const dim3 grid(blocks, units, p.B);
+    p.blocks = blocks;
+    p.units = units;
+    p.n_items = (int64_t)blocks * units * p.B;
+    const dim3 grid((unsigned)(p.n_items < 148 ? p.n_items : 148));       // one CTA per SM
     const bool bf = dtype == ATTN_B200_BF16;
-    if (D == 64) return bf ? launch<__nv_bfloat16, 64, false, false>(p, grid, st) : launch<__half, 64, false, false>(p, grid, st);
-    return bf ? launch<__nv_bfloat16, 128, false, false>(p, grid, st) : launch<__half, 128, false, false>(p, grid, st);
+    if (D == 64) return bf ? launch<__nv_bfloat16, 64, kWindow, false>(p, grid, st) : launch<__half, 64, kWindow, false>(p, grid, st);
+    return bf ? launch<__nv_bfloat16, 128, kWindow, false>(p, grid, st) : launch<__half, 128, kWindow, false>(p, grid, st);
 }
 
 void attend_prefix_plan(AttendParams& p) {
@@ -738,15 +973,18 @@ void attend_prefix_plan(AttendParams& p) {
 int attend_prefix_launch(const AttendParams& p, int D, int dtype, bool e4, cudaStream_t st) {
     const int64_t rows = (int64_t)p.B * (p.H / p.Hkv);
     const int64_t groups = p.key_split ? 1 : (rows + 2 * BM - 1) / (2 * BM);
-    if (groups > 65535 || p.Hkv > 65535) return ATTN_B200_ETOOLARGE;
-    const dim3 grid(p.splits, p.Hkv, (unsigned)groups);
-    const bool bf = dtype == ATTN_B200_BF16;
-    if (D == 64) {
-        if (e4) return bf ? launch<__nv_bfloat16, 64, true, true>(p, grid, st) : launch<__half, 64, true, true>(p, grid, st);
-        return bf ? launch<__nv_bfloat16, 64, true, false>(p, grid, st) : launch<__half, 64, true, false>(p, grid, st);
-    }
-    if (e4) return bf ? launch<__nv_bfloat16, 128, true, true>(p, grid, st) : launch<__half, 128, true, true>(p, grid, st);
-    return bf ? launch<__nv_bfloat16, 128, true, false>(p, grid, st) : launch<__half, 128, true, false>(p, grid, st);
+    if (p.splits * p.Hkv * groups > 0x7fffffffLL) return ATTN_B200_ETOOLARGE;
+    const dim3 grid((unsigned)(p.splits * p.Hkv * groups));
+    auto go = [&](auto hd, auto mode, auto e) -> int {
+        constexpr int HD = decltype(hd)::value, M = decltype(mode)::value;
+        constexpr bool E = decltype(e)::value;
+        return dtype == ATTN_B200_BF16 ? launch<__nv_bfloat16, HD, M, E>(p, grid, st) : launch<__half, HD, M, E>(p, grid, st);
+    };
+    auto with_mode = [&](auto hd, auto mode) { return e4 ? go(hd, mode, std::true_type{}) : go(hd, mode, std::false_type{}); };
+    auto with_dim = [&](auto hd) {
+        return p.key_split ? with_mode(hd, std::integral_constant<int, kPrefixSplit>{}) : with_mode(hd, std::integral_constant<int, kPrefixPair>{});
+    };
+    return D == 64 ? with_dim(std::integral_constant<int, 64>{}) : with_dim(std::integral_constant<int, 128>{});
 }
 
 }  // namespace attn

@@ -18,8 +18,10 @@ struct AttendParams {
     void* out;
     int64_t n_q_tokens, n_kv_tokens;
     int window, sinks, head_pairs;
+    int blocks, units;               // query blocks of the longest chunk, head units: set by the launcher
+    int64_t n_items;
     // prefix
-    float* parts;                    // [n_parts, B, H, D+2]
+    float* parts;                    // o [n_parts, B, H, D], then (m, l) [n_parts, B, H]
     int n_prefix, splits, key_split;
     const float *k_scale, *v_scale;
 };
@@ -29,7 +31,7 @@ bool attend_tc_supported(int D, int dtype, float scale);
 int attend_window_launch(AttendParams p, int max_q_len, int D, int dtype, cudaStream_t st);
 // partial rows of the shared prefix: sets p.splits and p.key_split from the sizes
 void attend_prefix_plan(AttendParams& p);
-inline int attend_prefix_parts(const AttendParams& p) { return p.splits * (p.key_split ? 2 : 1); }
+__host__ __device__ inline int attend_prefix_parts(const AttendParams& p) { return p.splits * (p.key_split ? 2 : 1); }
 int attend_prefix_launch(const AttendParams& p, int D, int dtype, bool e4m3, cudaStream_t st);
 
 }  // namespace attn

@@ -139,9 +139,10 @@ __device__ __forceinline__ void fold(const SpanParams& p, int b, int vh0, int ra
         float M = sn;
         for (int r = 0; r < S; ++r)
             for (int w = 0; w < wph; ++w) M = fmaxf(M, ld_cluster2(in_cta(ml0 + w * heads * 8, r)).x);
-        const float* rows = p.parts + ((int64_t)b * p.H + h) * (D + 2);
-        const int64_t row_step = (int64_t)p.B * p.H * (D + 2);
-        for (int k = 0; k < p.n_parts; ++k) M = fmaxf(M, rows[k * row_step + D]);
+        const int64_t set = (int64_t)p.B * p.H, bh = (int64_t)b * p.H + h;
+        const float2* pml = reinterpret_cast<const float2*>(p.parts + p.n_parts * set * D) + bh;
+        const float* po = p.parts + bh * D + d;
+        for (int k = 0; k < p.n_parts; ++k) M = fmaxf(M, pml[k * set].x);
         if (!(M > -INFINITY)) M = 0.f;           // nothing but -inf: 0 / 0 below, as the formula has it
         float w_new = fast_exp2(sn - M), den = w_new;
         float num = w_new * to_f32<T>(((const T*)p.v_new)[((int64_t)b * p.Hkv + hk) * D + d]);
@@ -153,10 +154,10 @@ __device__ __forceinline__ void fold(const SpanParams& p, int b, int vh0, int ra
                 num += e * ld_cluster(in_cta(part0 + w * part_stride, r));
             }
         for (int k = 0; k < p.n_parts; ++k) {
-            const float* row = rows + k * row_step;
-            const float e = fast_exp2(row[D] - M);
-            den += e * row[D + 1];
-            num += e * row[d];
+            const float2 v = pml[k * set];
+            const float e = fast_exp2(v.x - M);
+            den += e * v.y;
+            num += e * po[k * set * D];
         }
         ((T*)p.out)[((int64_t)b * p.H + h) * D + d] = from_f32<T>(num / den);
     }

@@ -13,7 +13,7 @@ struct SpanParams {
     const int32_t* prefix;              // slots of rows that every sequence sees before its own
     int n_prefix;
     void* out;
-    const float* parts;                 // [n_parts, B, H, D+2] rows [o[D], m (log2 domain), l] to fold in, or null
+    const float* parts;                 // to fold in, or null: o [n_parts, B, H, D], then (m (log2 domain), l) [n_parts, B, H]
     int n_parts;
     int B, H, Hkv, D;
     int64_t n_tokens, n_slots;          // entries of a per-token table; pool rows
