@@ -34,10 +34,12 @@ constexpr int BM = 128, BN = 128;
 constexpr int kSub = 128 * 128;                 // bytes of a [128 rows x 64 elements] 128-byte-swizzled sub-tile
 constexpr int kStages = 2;
 constexpr int kItems = 4;                       // items published ahead
-constexpr int kThreads = 512;                   // four warpgroups: softmax 0, softmax 1, {list, MMA, Q, Q}, {K, K, V, V}
-// Registers per thread.  setmaxnreg draws on the 512 * 128 the CTA was launched with.
-template <bool E4> struct Regs {
-    static constexpr int kSoftmax = E4 ? 192 : 208, kOther = E4 ? 48 : 56, kGather = E4 ? 80 : 40;
+// Warps 0-3 and 4-7 softmax, 8 item list, 9 MMA thread, 10 query tiles; 12-15 K and V, 32 rows of a tile each.  With
+// e4m3 rows 12-13 and 14-15 turn the raw K and V rows into fp16.
+// Registers per thread: setmaxnreg draws on the 512 * 128 that the CTA was launched with.
+constexpr int kThreads = 512;
+template <bool E4> struct Cfg {
+    static constexpr int kSoftmax = E4 ? 200 : 208, kOther = E4 ? 48 : 56, kGather = E4 ? 64 : 40;
     static_assert(8 * 32 * kSoftmax + 4 * 32 * kOther + 4 * 32 * kGather <= kThreads * 128, "register pool");
 };
 
@@ -64,7 +66,7 @@ template <int HD> struct Smem {
     signed char row_exp[2][BM];                         // bf16 queries over e4m3 rows: the power of two taken out of q
     Item item[kItems];
     alignas(8) unsigned long long item_full[kItems], item_empty[kItems];
-    unsigned long long q_full[2], q_empty[2], o_free[2];
+    unsigned long long q_full[2], q_empty[2], o_free[2], raw_full[2], raw_empty[2];
     unsigned long long s_full[2], p_half[2], p_full[2], o_full[2];
     unsigned long long k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
     unsigned int tmem_base;
@@ -84,6 +86,14 @@ __device__ __forceinline__ bool active(const Item& it, int w) { return it.je[w] 
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// Four rows of a two-dimensional tensor, one box (a row piece) each, to consecutive rows in shared memory; a row outside
+// the tensor arrives as zeros.  The tensor map's box is one row high.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, const int (&row)[4], void* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(smem_u32(bar))
+        : "memory");
 }
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -338,17 +348,23 @@ __device__ __forceinline__ bool softmax_rows(Smem<HD>& sm, int w, uint32_t s_add
     return true;
 }
 
-// Roles.  Warps 0-3 and 4-7 softmax, 8 item list, 9 MMA thread, 10 and 11 query tiles, 12-13 K, 14-15 V.  A window
-// launch is persistent: one CTA per SM takes every gridDim.x-th item, and the item list, the query tiles and the K/V
-// rings run ahead of the softmax, so that the set-up of an item hides under the one before it.  A prefix CTA has
-// one item.
+// A window launch is persistent: one CTA per SM takes every gridDim.x-th item, and the item list, the query tiles and
+// the K/V rings run ahead of the softmax, so that the set-up of an item hides under the one before it.  A prefix
+// CTA has one item.
+//
+// K and V rows are gathered by TMA (tile::gather4): a lane owns four rows of a tile, fetches and checks their slots one
+// tile ahead and issues one copy per 128 bytes of row; a slot outside the pool becomes the row behind its last one, which
+// arrives as zeros.  Issuing is the bound (about 45 ns per copy of a warp, whatever other warps do): one warp per stream
+// took 3 us for a tile, so four warps share both.  (Copied by 128 threads with cp.async, 16 bytes at a time, a tile took
+// 2 to 4 us beside the softmax warps, whose issue slots those copies also take.)
 enum Mode { kWindow, kPrefixPair, kPrefixSplit };      // kPrefixSplit: AttendParams::key_split
 template <typename T, int HD, int kMode, bool E4>
 __global__ void __launch_bounds__(kThreads, 1)
-attend_tc_kernel(const AttendParams p) {
+attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                 const __grid_constant__ CUtensorMap map_v, const AttendParams p) {
     constexpr bool kPrefix = kMode != kWindow, key_split = kMode == kPrefixSplit;
     using MT = typename std::conditional<E4, __half, T>::type;       // e4m3 rows are multiplied as fp16
-    using R = Regs<E4>;
+    using R = Cfg<E4>;
     constexpr int kTileBytes = Smem<HD>::kTile;
     constexpr int QC = HD / 8;                                       // 16-byte chunks of a query row
     extern __shared__ unsigned char smem_raw[];
@@ -360,10 +376,12 @@ attend_tc_kernel(const AttendParams p) {
     if (threadIdx.x == 0) {
         for (int i = 0; i < kItems; ++i) {
             mbar_init(&sm.item_full[i], 1);
-            mbar_init(&sm.item_empty[i], 15);       // one lane of every warp but the list's own
+            mbar_init(&sm.item_empty[i], E4 ? 13 : 14);       // one lane of every warp that reads the list
         }
         for (int w = 0; w < 2; ++w) {
-            mbar_init(&sm.q_full[w], kPrefix ? 128 : 32);
+            mbar_init(&sm.q_full[w], kPrefix ? 128 : 1);
+            mbar_init(&sm.raw_full[w], 1);
+            mbar_init(&sm.raw_empty[w], 64);
             mbar_init(&sm.q_empty[w], 1);
             mbar_init(&sm.o_free[w], 128);
             mbar_init(&sm.s_full[w], 1);
@@ -372,9 +390,9 @@ attend_tc_kernel(const AttendParams p) {
             mbar_init(&sm.o_full[w], 1);
         }
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(&sm.k_full[s], 64);
+            mbar_init(&sm.k_full[s], E4 ? 64 : 4);
             mbar_init(&sm.k_empty[s], 1);
-            mbar_init(&sm.v_full[s], 64);
+            mbar_init(&sm.v_full[s], E4 ? 64 : 4);
             mbar_init(&sm.v_empty[s], 1);
         }
         sm.any_bad = 0;
@@ -429,7 +447,7 @@ attend_tc_kernel(const AttendParams p) {
         }
         return Rows{((it.q_beg + row) * p.H + it.head[w]) * HD, it.n_rows - row, 0, 1, p.H * HD};
     };
-    // A warp copies query rows r0 .. r0 + n - 1 of a tile into its swizzled place, whole rows at a time
+    // prefix: a warp copies query rows r0 .. r0 + n - 1 of a tile into its swizzled place, whole rows at a time
     auto load_q = [&](const Item& it, int w, int r0, int n) {
         constexpr int kAtOnce = 32 / QC;
         const int cc = lane % QC, rr = lane / QC;
@@ -473,113 +491,160 @@ attend_tc_kernel(const AttendParams p) {
         mbar_arrive(&sm.q_full[w]);
     };
 
-    if (warp >= 12) {
-        // ------------------------------------------------------------------ gather: 64 threads K, 64 threads V
+    // Slots of an item's tiles, four rows from `r0` of a tile per lane, fetched ahead of their use
+    struct Slots {
+        const int32_t* table;
+        int w0, tiles, sinks, skip, n_slots;
+        __device__ __forceinline__ Slots(const AttendParams& p, const Item& it)
+            : table(p.table + it.beg), w0(it.w0), tiles(it.tiles), sinks(it.sinks), skip(it.first - it.sinks), n_slots((int)p.n_slots) {}
+        __device__ __forceinline__ void fetch(int j, int r0, int (&x)[4]) const {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = r0 + i, u = tile_base(w0, j) + r;
+                x[i] = j < tiles && r < BN && r < tile_keys(w0, j) ? __ldg(table + (u < sinks ? u : u + skip)) : -1;
+            }
+        }
+    };
+    // Slots -> rows to gather; `mark`: notes which rows of the tile (the CTA's t-th) there are none for.  bad[t & 3] is
+    // read until the tile's P is there, which the MMA thread waits for before it issues anything of two tiles later
+    // and so before the release that lets the tile after next but one in.
+    auto to_rows = [&](const Slots& sl, int j, int t, int r0, const int (&x)[4], int (&row)[4], bool mark) {
+        bool bad = false;
+        uint32_t bytes = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool in = x[i] >= 0 && x[i] < sl.n_slots;
+            bad |= !in && r0 + i < tile_keys(sl.w0, j);
+            bytes |= in ? 0u : 1u << (8 * i);
+            row[i] = in ? x[i] : sl.n_slots;
+        }
+        if (mark && (E4 || lane < 8)) {
+            *reinterpret_cast<uint32_t*>(&sm.bad[t & 3][r0]) = bytes;
+            if (bad) {
+                sm.any_bad = 1;
+                if (p.err_flag) atomicOr(p.err_flag, ATTN_B200_FLAG_BAD_SLOT);
+            }
+        }
+    };
+
+    if (E4 && warp >= 12) {
+        // ------------------------------------------------------------------ e4m3 rows: 64 threads K, 64 threads V
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::kGather));
-        constexpr int kRow = E4 ? HD : 2 * HD;                              // bytes of a head's row in the pool
-        constexpr int CPR = kRow / 16, RPP = 64 / CPR, PASSES = BN / RPP;   // chunks of a row; rows per pass of 64 threads
-        const int tid = threadIdx.x - 384, t64 = tid & 63;
-        const bool v_stream = tid >= 64;
+        constexpr int CPR = HD / 16, RPP = 64 / CPR, PASSES = BN / RPP;     // 16-byte chunks of a raw row; rows per pass of 64 threads
+        const int v = warp >= 14, t64 = threadIdx.x & 63;
+        const bool fetches = (warp & 1) == 0;                               // the stream's first warp gathers
         const int c = t64 % CPR, rsub = t64 / CPR;
-        unsigned long long* full = v_stream ? sm.v_full : sm.k_full;
-        unsigned long long* empty = v_stream ? sm.v_empty : sm.k_empty;
-        unsigned char (*stage)[kTileBytes] = v_stream ? sm.v : sm.k;
-        const uint32_t raw = smem_u32(sm.extra[v_stream]) + t64 * 16;       // e4m3: this thread's chunk of pass 0
-        const int64_t row_bytes = (int64_t)p.Hkv * kRow;
-        int g = 0;                                                          // tiles of earlier items
-        for (int n = 0;; ++n) {
-            const Item* const ip = next_item(n);
-            if (__any_sync(0xffffffffu, !ip)) break;
-            const Item& it = *ip;
-            const int w0 = it.w0, tiles = it.tiles, sinks = it.sinks, skip = it.first - it.sinks;
-            const int32_t* const table = p.table + it.beg;
-            const char* const base = (const char*)(v_stream ? p.v_cache : p.k_cache) + (int64_t)it.hk * kRow + c * 16;
-            // The CPR threads of a row group need the same PASSES slots: thread c fetches and checks those of
-            // passes c and c + CPR (one tile ahead), the copies take them by shuffle.
-            int ahead[2];
-            auto fetch = [&](int j) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int r = (c + CPR * i) * RPP + rsub, u = tile_base(w0, j) + r;
-                    ahead[i] = j < tiles && r < tile_keys(w0, j) ? __ldg(table + (u < sinks ? u : u + skip)) : -1;
-                }
+        unsigned long long* full = v ? sm.v_full : sm.k_full;
+        unsigned long long* empty = v ? sm.v_empty : sm.k_empty;
+        const CUtensorMap* const map = v ? &map_v : &map_k;
+        const uint32_t raw = smem_u32(sm.extra[v]);
+        int issued = 0;
+        if (const Item* const ip = next_item(0)) {                          // prefix only: one item
+            const Slots sl(p, *ip);
+            const int tiles = sl.tiles, x0 = ip->hk * HD;
+            int ahead[4], cur[4];
+            auto gather = [&](int j) {                                      // raw rows of tile j, whose slots are in `ahead`
+                to_rows(sl, j, j, lane * 4, ahead, cur, false);
+                if (lane == 0) mbar_expect_tx(&sm.raw_full[v], BN * HD);
+                __syncwarp();
+                tma_gather4(raw + lane * 4 * HD, map, x0, cur, &sm.raw_full[v]);
+                ++issued;
             };
-            // destination of row q RPP + rsub, chunk c: the row's low three bits are those of q RPP + rsub, so
-            // there are at most two swizzle terms per thread and everything else is a compile-time offset
-            const uint32_t swz0 = rsub * 128 + ((((uint32_t)c & 7) ^ (uint32_t)(rsub & 7)) << 4);
-            const uint32_t swz1 = rsub * 128 + ((((uint32_t)c & 7) ^ (uint32_t)((RPP + rsub) & 7)) << 4);
-            auto copy = [&](uint32_t dst, const int (&sl)[2]) {
-                const uint32_t d0 = dst + swz0, d1 = dst + swz1;
-#pragma unroll
-                for (int q = 0; q < PASSES; ++q) {
-                    const int v = __shfl_sync(0xffffffffu, sl[q / CPR], q % CPR, CPR);
-                    cp16(E4 ? dst + q * 1024 : ((q & 1) ? d1 : d0) + q * (RPP * 128), base + (int64_t)(v >= 0 ? v : 0) * row_bytes, v >= 0 ? 16 : 0);
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-            auto checked = [&](int (&sl)[2]) {       // slots outside the pools become -1
-#pragma unroll
-                for (int i = 0; i < 2; ++i) sl[i] = ahead[i] >= 0 && ahead[i] < p.n_slots ? ahead[i] : -1;
-            };
-            // bad[tile & 3]: written before the tile is published and read until its P is there, which the MMA thread
-            // waits for before it issues anything of two tiles later and so before the release that lets the
-            // tile after next but one in
-            auto mark = [&](int j, const int (&sl)[2]) {
-                bool bad = false;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int r = (c + CPR * i) * RPP + rsub;
-                    bad |= r < tile_keys(w0, j) && sl[i] < 0;
-                    if (!v_stream) sm.bad[(g + j) & 3][r] = sl[i] < 0;
-                }
-                if (bad) {
-                    if (!v_stream) sm.any_bad = 1;
-                    if (p.err_flag) atomicOr(p.err_flag, ATTN_B200_FLAG_BAD_SLOT);
-                }
-            };
-            fetch(0);
-            int sl[2];
-            checked(sl);
-            if (E4) copy(raw, sl);        // the raw rows of a tile travel while the tile before it is still in use
-            bool ok = true;
+            if (fetches) {
+                sl.fetch(0, lane * 4, ahead);
+                gather(0);
+            }
             for (int j = 0; j < tiles; ++j) {
-                const int t = g + j, s = t % kStages;
-                fetch(j + 1);
-                if (t >= kStages) ok = mbar_wait(&empty[s], ((t - kStages) / kStages) & 1, wc);
+                const int s = j % kStages;
+                int mine[4] = {ahead[0], ahead[1], ahead[2], ahead[3]};
+                if (fetches) sl.fetch(j + 1, lane * 4, ahead);
+                bool ok = mbar_wait(&sm.raw_full[v], j & 1, wc);
+                if (ok && j >= kStages) ok = mbar_wait(&empty[s], ((j - kStages) / kStages) & 1, wc);
                 if (!__all_sync(0xffffffffu, ok)) break;
-                mark(j, sl);
-                if constexpr (!E4) {
-                    copy(smem_u32(stage[s]) + (c >> 3) * kSub, sl);
-                    asm volatile("cp.async.wait_group 0;" ::: "memory");
-                } else {
-                    asm volatile("cp.async.wait_group 0;" ::: "memory");
-                    // 16 codes -> chunks 2 c and 2 c + 1 of the row in fp16; a thread reads what it copied itself
-                    const uint32_t dst = smem_u32(stage[s]) + (c >> 2) * kSub;
+                if (fetches) to_rows(sl, j, j, lane * 4, mine, cur, !v);
+                // 16 codes -> chunks 2 c and 2 c + 1 of the row in fp16
+                const uint32_t dst = smem_u32(v ? sm.v[s] : sm.k[s]) + (c >> 2) * kSub;
 #pragma unroll 4
-                    for (int q = 0; q < PASSES; ++q) {
-                        const int r = q * RPP + rsub;
-                        const uint4 x = ld_shared16(raw + q * 1024);
-                        __half2 h[8];
-                        e4m3x4_to_half2x2(x.x, h[0], h[1]);
-                        e4m3x4_to_half2x2(x.y, h[2], h[3]);
-                        e4m3x4_to_half2x2(x.z, h[4], h[5]);
-                        e4m3x4_to_half2x2(x.w, h[6], h[7]);
-                        const uint32_t* u = reinterpret_cast<const uint32_t*>(h);
-                        const uint32_t at = dst + r * 128;
-                        st_shared16(at + ((((2 * c) & 7) ^ (r & 7)) << 4), u[0], u[1], u[2], u[3]);
-                        st_shared16(at + ((((2 * c + 1) & 7) ^ (r & 7)) << 4), u[4], u[5], u[6], u[7]);
-                    }
+                for (int q = 0; q < PASSES; ++q) {
+                    const int r = q * RPP + rsub;
+                    const uint4 x = ld_shared16(raw + r * HD + c * 16);
+                    __half2 h[8];
+                    e4m3x4_to_half2x2(x.x, h[0], h[1]);
+                    e4m3x4_to_half2x2(x.y, h[2], h[3]);
+                    e4m3x4_to_half2x2(x.z, h[4], h[5]);
+                    e4m3x4_to_half2x2(x.w, h[6], h[7]);
+                    const uint32_t* u = reinterpret_cast<const uint32_t*>(h);
+                    const uint32_t at = dst + r * 128;
+                    st_shared16(at + ((((2 * c) & 7) ^ (r & 7)) << 4), u[0], u[1], u[2], u[3]);
+                    st_shared16(at + ((((2 * c + 1) & 7) ^ (r & 7)) << 4), u[4], u[5], u[6], u[7]);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(&full[s]);
-                checked(sl);
-                if (E4 && j + 1 < tiles) copy(raw, sl);
+                mbar_arrive(&sm.raw_empty[v]);
+                if (fetches && j + 1 < tiles) {            // the next raw rows travel while this tile is in use
+                    if (!__all_sync(0xffffffffu, mbar_wait(&sm.raw_empty[v], j & 1, wc))) break;
+                    gather(j + 1);
+                }
             }
-            if (!__all_sync(0xffffffffu, ok)) break;
+            done_with(0);
+        }
+        if (fetches && lane == 0 && sm.box.abort && issued > 0) {      // a copy still in flight gets a bounded time to land
+            const long long t0 = clock64();
+            while (!mbar_try(&sm.raw_full[v], (issued - 1) & 1) && clock64() - t0 < WAIT_CYCLES) {}
+        }
+    } else if (!E4 && warp >= 12) {
+        // ------------------------------------------------------------------ K and V rows 32 (warp - 12) .. + 31 of every tile
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::kGather));
+        const int r0 = (warp - 12) * 32 + (lane & 7) * 4;                   // lanes 0-7 gather, four rows each
+        const uint32_t at = r0 * 128;
+        int g = 0, issued_k = 0, issued_v = 0;
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+            const Item* const ip = next_item(n);
+            if (__any_sync(0xffffffffu, !ip)) break;
+            const Slots sl(p, *ip);
+            const int x0 = ip->hk * HD, tiles = sl.tiles;
+            int ahead[4];
+            sl.fetch(0, r0, ahead);
+            for (int j = 0; j < tiles; ++j) {
+                const int t = g + j, s = t % kStages;
+                const uint32_t ph = ((t - kStages) / kStages) & 1;
+                int row[4], cur[4] = {ahead[0], ahead[1], ahead[2], ahead[3]};
+                sl.fetch(j + 1, r0, ahead);
+                if (t >= kStages) ok = mbar_wait(&sm.k_empty[s], ph, wc);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                to_rows(sl, j, t, r0, cur, row, true);
+                __syncwarp();                           // the notes of all lanes stand before lane 0 arrives
+                if (lane == 0) mbar_expect_tx(&sm.k_full[s], kTileBytes / 4);
+                __syncwarp();
+                if (lane < 8) {
+#pragma unroll
+                    for (int c = 0; c < HD / 64; ++c) tma_gather4(smem_u32(sm.k[s]) + at + c * kSub, &map_k, x0 + c * 64, row, &sm.k_full[s]);
+                }
+                ++issued_k;
+                __syncwarp();
+                if (t >= kStages) ok = mbar_wait(&sm.v_empty[s], ph, wc);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                if (lane == 0) mbar_expect_tx(&sm.v_full[s], kTileBytes / 4);
+                __syncwarp();
+                if (lane < 8) {
+#pragma unroll
+                    for (int c = 0; c < HD / 64; ++c) tma_gather4(smem_u32(sm.v[s]) + at + c * kSub, &map_v, x0 + c * 64, row, &sm.v_full[s]);
+                }
+                ++issued_v;
+                __syncwarp();
+            }
+            if (!ok) break;
             g += tiles;
             done_with(n);
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (lane == 0 && sm.box.abort) {                 // copies still in flight get a bounded time to land
+            const long long t0 = clock64();
+            for (int t = issued_k > kStages ? issued_k - kStages : 0; t < issued_k; ++t)
+                while (!mbar_try(&sm.k_full[t % kStages], (t / kStages) & 1) && clock64() - t0 < WAIT_CYCLES) {}
+            for (int t = issued_v > kStages ? issued_v - kStages : 0; t < issued_v; ++t)
+                while (!mbar_try(&sm.v_full[t % kStages], (t / kStages) & 1) && clock64() - t0 < WAIT_CYCLES) {}
+        }
     } else if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::kOther));
         if (warp == 8) {
@@ -723,21 +788,35 @@ attend_tc_kernel(const AttendParams p) {
                 }
             }
             __syncwarp();
-        } else {
-            // -------------------------------------------------------------- window: query tile of warpgroup `w`
-            const int w = warp - 10;
-            int uses = 0;
-            for (int n = 0;; ++n) {
+        } else if (!kPrefix && warp == 10) {
+            // -------------------------------------------------------------- query tiles
+            int uses[2] = {0, 0};
+            bool ok = true;
+            for (int n = 0; ok; ++n) {
                 const Item* const ip = next_item(n);
                 if (__any_sync(0xffffffffu, !ip)) break;
                 const Item& it = *ip;
-                if (!kPrefix && active(it, w)) {
-                    const bool ok = uses == 0 || mbar_wait(&sm.q_empty[w], (uses - 1) & 1, wc);
-                    if (!__all_sync(0xffffffffu, ok)) break;
-                    load_q(it, w, 0, BM);
-                    ++uses;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    if (!ok || !active(it, w)) continue;
+                    ok = uses[w] == 0 || mbar_wait(&sm.q_empty[w], (uses[w] - 1) & 1, wc);
+                    if (!(ok = __all_sync(0xffffffffu, ok))) continue;
+                    ++uses[w];
+                    if (lane == 0) {
+                        // rows past the chunk's end are another sequence's (or zeros past the tensor): computed, not stored
+                        mbar_expect_tx(&sm.q_full[w], kTileBytes);
+#pragma unroll
+                        for (int c = 0; c < HD / 64; ++c)
+                            tma_load_2d(sm.q[w] + c * kSub, &map_q, it.head[w] * HD + c * 64, (int)(it.q_beg + it.row0[w]), &sm.q_full[w]);
+                    }
+                    __syncwarp();
                 }
-                done_with(n);
+                if (ok) done_with(n);
+            }
+            if (lane == 0 && sm.box.abort) {
+                const long long t0 = clock64();
+                for (int w = 0; w < 2; ++w)
+                    if (uses[w] > 0) while (!mbar_try(&sm.q_full[w], (uses[w] - 1) & 1) && clock64() - t0 < WAIT_CYCLES) {}
             }
         }
     } else {
@@ -892,8 +971,8 @@ __global__ void zero_rows_kernel(void* out, const int32_t* q_offsets, const int3
 // host side
 // ---------------------------------------------------------------------------------------------
 // Launch as a programmatic dependent: the kernels wait (griddepcontrol.wait) before they read anything.
-template <typename... A>
-int launch_dependent(void (*kernel)(A...), dim3 grid, int threads, int smem, cudaStream_t st, A... args) {
+template <typename... K, typename... A>
+int launch_dependent(void (*kernel)(K...), dim3 grid, int threads, int smem, cudaStream_t st, const A&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
@@ -909,6 +988,30 @@ int launch_dependent(void (*kernel)(A...), dim3 grid, int threads, int smem, cud
 
 static_assert(sizeof(Smem<128>) + 1024 <= 227 * 1024, "shared memory");
 
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encoder() {
+    static const EncodeTiled fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<EncodeTiled>(f) : nullptr;
+    }();
+    return fn;
+}
+// [rows, cols] row-major; boxes of `width` elements x `height` rows
+int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int elem_bytes, int width, int height, bool swizzle) {
+    const EncodeTiled fn = encoder();
+    if (!fn) return (int)cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(cols * elem_bytes)};
+    const cuuint32_t box[2] = {(cuuint32_t)width, (cuuint32_t)height}, step[2] = {1, 1};
+    // the copies move bits: every 16-bit type is taken as fp16
+    const CUresult r = fn(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
+                          strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
 template <typename T, int HD, int kMode, bool E4>
 int launch(const AttendParams& p, dim3 grid, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
@@ -922,7 +1025,18 @@ int launch(const AttendParams& p, dim3 grid, cudaStream_t st) {
             return (int)e;
         ready.fetch_or(1ull << dev, std::memory_order_release);
     }
-    return launch_dependent(attend_tc_kernel<T, HD, kMode, E4>, grid, kThreads, smem, st, p);
+    CUtensorMap mq, mk, mv;
+    const int64_t cols = (int64_t)p.Hkv * HD;
+    int rc;
+    if ((rc = make_map(&mk, p.k_cache, p.n_slots, cols, E4 ? 1 : 2, E4 ? HD : 64, 1, !E4)) ||
+        (rc = make_map(&mv, p.v_cache, p.n_slots, cols, E4 ? 1 : 2, E4 ? HD : 64, 1, !E4)))
+        return rc;
+    if (kMode == kWindow) {
+        if ((rc = make_map(&mq, p.q, p.n_q_tokens, (int64_t)p.H * HD, 2, 64, BM, true))) return rc;
+    } else {
+        mq = mk;               // not used
+    }
+    return launch_dependent(attend_tc_kernel<T, HD, kMode, E4>, grid, kThreads, smem, st, mq, mk, mv, p);
 }
 
 }  // namespace

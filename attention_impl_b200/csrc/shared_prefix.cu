@@ -72,7 +72,7 @@ extern "C" int attn_b200_shared_prefix_decode(const void* q, const void* k_new, 
     p.v_scale = e4 ? v_scale : nullptr;
     p.err_flag = err_flag;
     const bool aligned = (((uintptr_t)q | (uintptr_t)k_new | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0;
-    if (aligned && on_tensor_cores(D, q_dtype, kv_dtype, scale, n_prefix)) {
+    if (aligned && n_slots > 0 && on_tensor_cores(D, q_dtype, kv_dtype, scale, n_prefix)) {
         AttendParams a = plan(B, H, n_kv_heads, n_prefix);
         const int parts = attend_prefix_parts(a);
         if ((uintptr_t)workspace % 16 || !workspace || workspace_bytes < (size_t)parts * B * H * (D + 2) * sizeof(float))

@@ -101,7 +101,7 @@ extern "C" int attn_b200_paged_window_prefill(const void* q, const void* k_cache
     p.n_q_tokens = n_q_tokens; p.n_kv_tokens = n_kv_tokens;
     p.window = window; p.sinks = n_sinks;
     cudaStream_t st = (cudaStream_t)stream;
-    if (!force_generic && attend_tc_supported(D, dtype, scale) &&
+    if (!force_generic && n_slots > 0 && attend_tc_supported(D, dtype, scale) &&
         (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) == 0)
         return attend_window_launch(p, max_q_len, D, dtype, st);
     switch (dtype) {
