@@ -120,46 +120,99 @@ __device__ __forceinline__ int64_t slot_of(const SpanParams& p, const Span& s, i
     return slot;
 }
 
-// Folds the workers' partial results, the shared rows' partial results and the current token, and writes
-// O.  Every CTA of the cluster has, per warp, a partial row [heads][D] at `part` (warp stride `part_stride`
-// bytes) and (m, l) pairs [heads of a warp] at `ml`; s_new [slot][heads] are the current token's scores.
-template <typename T>
-__device__ __forceinline__ void fold(const SpanParams& p, int b, int vh0, int rank, uint32_t part, uint32_t part_stride, uint32_t ml,
-                                     const float* s_new, int heads, int per_set) {
-    const int hpc = 1 << p.hpc_log2, wph = kWarps >> p.hpc_log2, S = p.splits, D = p.D;
-    const int G = p.H / p.Hkv;
-    const int items = hpc * heads * D;
-    for (int i = rank * (kWarps * 32) + threadIdx.x; i < items; i += S * kWarps * 32) {
-        const int d = i % D, gh = i / D, g = gh % heads, slot = gh / heads;
-        const int vh = vh0 + slot, hk = vh / p.n_sets, gq = (vh - hk * p.n_sets) * per_set + g;
-        if (hk >= p.Hkv || gq >= G) continue;
-        const int h = hk * G + gq;
-        const float sn = s_new[slot * heads + g];
-        const uint32_t ml0 = ml + (slot * wph * heads + g) * 8, part0 = part + slot * wph * part_stride + (g * D + d) * 4;
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void add4(float4& a, float w, const float4& x) {
+    a.x += w * x.x;
+    a.y += w * x.y;
+    a.z += w * x.z;
+    a.w += w * x.w;
+}
+
+constexpr int kMaxSplits = 16;
+// Weights of the partial results a CTA folds: per head of the CTA, one per worker (CTA of the cluster x warp of the
+// KV head), the current token's, and what turns a shared-row partial's 2^m into its weight
+struct FoldWeights {
+    float worker[kWarps * 8][kMaxSplits];   // heads of the CTA x workers: at most (4 x 8) x 16 or (1 x 8) x 64
+    float fresh[kWarps * 8], top[kWarps * 8], inv[kWarps * 8];
+};
+
+// Folds the workers' partial results, the shared rows' partial results and the current token, and writes O.
+// Every CTA of the cluster has, per warp, a partial row [heads][D] at `part` (warp stride `part_stride` bytes) and
+// (m, l) pairs [heads of a warp] at `ml`; s_new [slot][heads] are the current token's scores.  A warp forms the weights
+// of a head with a worker per lane, then every thread sums four output entries, its loads from the other CTAs independent.
+template <typename T, int D>
+__device__ __forceinline__ void fold(const SpanParams& p, FoldWeights& fw, int b, int vh0, int rank, uint32_t part, uint32_t part_stride,
+                                     uint32_t ml, const float* s_new, int heads) {
+    const int hpc = 1 << p.hpc_log2, wph_log2 = 2 - p.hpc_log2, S = p.splits, workers = S << wph_log2;
+    const int G = p.H / p.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float* const weight = &fw.worker[0][0];                  // [hpc * heads][workers]
+    const int64_t set = (int64_t)p.B * p.H;
+    const float2* const pml = reinterpret_cast<const float2*>(p.parts + p.n_parts * set * D) + (int64_t)b * p.H;
+    auto head_of = [&](int gh) -> int {                      // query head of this CTA's gh-th, or -1
+        const int slot = gh / heads, vh = vh0 + slot, hk = vh / p.n_sets, g = (vh - hk * p.n_sets) * 8 + gh - slot * heads;
+        return hk < p.Hkv && g < G ? hk * G + g : -1;
+    };
+    for (int gh = warp; gh < hpc * heads; gh += kWarps) {
+        const int h = head_of(gh), slot = gh / heads;
+        if (h < 0) continue;
+        const float sn = s_new[gh];
+        float2 v[2];
         float M = sn;
-        for (int r = 0; r < S; ++r)
-            for (int w = 0; w < wph; ++w) M = fmaxf(M, ld_cluster2(in_cta(ml0 + w * heads * 8, r)).x);
-        const int64_t set = (int64_t)p.B * p.H, bh = (int64_t)b * p.H + h;
-        const float2* pml = reinterpret_cast<const float2*>(p.parts + p.n_parts * set * D) + bh;
-        const float* po = p.parts + bh * D + d;
-        for (int k = 0; k < p.n_parts; ++k) M = fmaxf(M, pml[k * set].x);
-        if (!(M > -INFINITY)) M = 0.f;           // nothing but -inf: 0 / 0 below, as the formula has it
-        float w_new = fast_exp2(sn - M), den = w_new;
-        float num = w_new * to_f32<T>(((const T*)p.v_new)[((int64_t)b * p.Hkv + hk) * D + d]);
-        for (int r = 0; r < S; ++r)
-            for (int w = 0; w < wph; ++w) {
-                const float2 v = ld_cluster2(in_cta(ml0 + w * heads * 8, r));
-                const float e = fast_exp2(v.x - M);
-                den += e * v.y;
-                num += e * ld_cluster(in_cta(part0 + w * part_stride, r));
-            }
-        for (int k = 0; k < p.n_parts; ++k) {
-            const float2 v = pml[k * set];
-            const float e = fast_exp2(v.x - M);
-            den += e * v.y;
-            num += e * po[k * set * D];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int w = lane + 32 * i, warp_of = (slot << wph_log2) + (w & ((1 << wph_log2) - 1));
+            v[i] = make_float2(-INFINITY, 0.f);
+            if (w < workers) v[i] = ld_cluster2(in_cta(ml + (warp_of * heads + gh - slot * heads) * 8, w >> wph_log2));
+            M = fmaxf(M, v[i].x);
         }
-        ((T*)p.out)[((int64_t)b * p.H + h) * D + d] = from_f32<T>(num / den);
+        for (int k = lane; k < p.n_parts; k += 32) M = fmaxf(M, pml[k * set + h].x);
+        M = group_max<32>(M);
+        if (!(M > -INFINITY)) M = 0.f;                       // nothing but -inf: 0 / 0 below, as the formula has it
+        float e[2], den = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            e[i] = fast_exp2(v[i].x - M);
+            den += e[i] * v[i].y;
+        }
+        for (int k = lane; k < p.n_parts; k += 32) {
+            const float2 x = pml[k * set + h];
+            den += fast_exp2(x.x - M) * x.y;
+        }
+        const float fresh = fast_exp2(sn - M);
+        const float inv = 1.f / (group_sum<32>(den) + fresh);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (lane + 32 * i < workers) weight[gh * workers + lane + 32 * i] = e[i] * inv;
+        if (lane == 0) {
+            fw.fresh[gh] = fresh * inv;
+            fw.top[gh] = M;
+            fw.inv[gh] = inv;
+        }
+    }
+    __syncthreads();
+    const int items = hpc * heads * (D / 4);
+    for (int i = rank * (kWarps * 32) + threadIdx.x; i < items; i += S * kWarps * 32) {
+        const int d = (i % (D / 4)) * 4, gh = i / (D / 4), slot = gh / heads, h = head_of(gh);
+        if (h < 0) continue;
+        const T* vn = (const T*)p.v_new + ((int64_t)b * p.Hkv + h / G) * D + d;
+        const float f = fw.fresh[gh];
+        float4 o = make_float4(f * to_f32<T>(vn[0]), f * to_f32<T>(vn[1]), f * to_f32<T>(vn[2]), f * to_f32<T>(vn[3]));
+        const uint32_t part0 = part + (slot << wph_log2) * part_stride + ((gh - slot * heads) * D + d) * 4;
+#pragma unroll 4
+        for (int w = 0; w < workers; ++w)
+            add4(o, weight[gh * workers + w], ld_cluster4(in_cta(part0 + (w & ((1 << wph_log2) - 1)) * part_stride, w >> wph_log2)));
+        const float4* po = reinterpret_cast<const float4*>(p.parts + ((int64_t)b * p.H + h) * D + d);
+#pragma unroll 4
+        for (int k = 0; k < p.n_parts; ++k) add4(o, fast_exp2(pml[k * set + h].x - fw.top[gh]) * fw.inv[gh], po[k * set * (D / 4)]);
+        T* out = (T*)p.out + ((int64_t)b * p.H + h) * D + d;
+        out[0] = from_f32<T>(o.x);
+        out[1] = from_f32<T>(o.y);
+        out[2] = from_f32<T>(o.z);
+        out[3] = from_f32<T>(o.w);
     }
 }
 
@@ -174,7 +227,7 @@ template <int D, bool E4> struct Ring {
 };
 
 template <typename T, int D, bool E4>
-__global__ void __launch_bounds__(kWarps * 32, (227 * 1024 / (Ring<D, E4>::kBytes + 2048) < 4 ? 227 * 1024 / (Ring<D, E4>::kBytes + 2048) : 4))
+__global__ void __launch_bounds__(kWarps * 32, (227 * 1024 / (Ring<D, E4>::kBytes + 4096) < 4 ? 227 * 1024 / (Ring<D, E4>::kBytes + 4096) : 4))
 span_decode_kernel(const SpanParams p) {
     using R = Ring<D, E4>;
     using MT = typename std::conditional<E4, __half, T>::type;   // e4m3 rows are multiplied as fp16
@@ -183,6 +236,7 @@ span_decode_kernel(const SpanParams p) {
     extern __shared__ __align__(16) unsigned char ring_raw[];
     __shared__ float2 s_ml[kWarps * 8];
     __shared__ float s_new[kWarps * 8];
+    __shared__ FoldWeights s_fold;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n = lane >> 2, c = lane & 3;
@@ -416,8 +470,8 @@ span_decode_kernel(const SpanParams p) {
     if (p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     cluster_sync();
-    fold<T>(p, b, vh0, rank, (uint32_t)__cvta_generic_to_shared(ring_raw), R::kWarpBytes, (uint32_t)__cvta_generic_to_shared(s_ml),
-            s_new, heads, 8);
+    fold<T, D>(p, s_fold, b, vh0, rank, (uint32_t)__cvta_generic_to_shared(ring_raw), R::kWarpBytes, (uint32_t)__cvta_generic_to_shared(s_ml),
+               s_new, heads);
     cluster_sync();              // nobody leaves while its shared memory is still read
 }
 
