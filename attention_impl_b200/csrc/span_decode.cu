@@ -143,7 +143,7 @@ struct FoldWeights {
 // Folds the workers' partial results, the shared rows' partial results and the current token, and writes O.
 // Every CTA of the cluster has, per warp, a partial row [heads][D] at `part` (warp stride `part_stride` bytes) and
 // (m, l) pairs [heads of a warp] at `ml`; s_new [slot][heads] are the current token's scores.  A warp forms the weights
-// of a head with a worker per lane, then every thread sums four output entries, its loads from the other CTAs independent.
+// of a head with a worker per lane, then the threads sum four output entries each, their loads from the other CTAs independent.
 template <typename T, int D>
 __device__ __forceinline__ void fold(const SpanParams& p, FoldWeights& fw, int b, int vh0, int rank, uint32_t part, uint32_t part_stride,
                                      uint32_t ml, const float* s_new, int heads) {
@@ -194,20 +194,32 @@ __device__ __forceinline__ void fold(const SpanParams& p, FoldWeights& fw, int b
         }
     }
     __syncthreads();
-    const int items = hpc * heads * (D / 4);
-    for (int i = rank * (kWarps * 32) + threadIdx.x; i < items; i += S * kWarps * 32) {
-        const int d = (i % (D / 4)) * 4, gh = i / (D / 4), slot = gh / heads, h = head_of(gh);
-        if (h < 0) continue;
+    // Where there are more threads than output vectors, 2^k threads of a warp share one and split its partial results.
+    const int items = hpc * heads * (D / 4), threads = S * kWarps * 32;
+    int share = 1;
+    while (share < 32 && items * share * 2 <= threads) share *= 2;
+    const int first = rank * (kWarps * 32) + threadIdx.x, sub = first & (share - 1);
+    for (int i = first / share; i - (lane / share) < items; i += threads / share) {       // whole warps together
+        const int d = (i % (D / 4)) * 4, gh = i / (D / 4), slot = gh / heads, h = i < items ? head_of(gh) : -1;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (h >= 0) {
+            const uint32_t part0 = part + (slot << wph_log2) * part_stride + ((gh - slot * heads) * D + d) * 4;
+#pragma unroll 4
+            for (int w = sub; w < workers; w += share)
+                add4(o, weight[gh * workers + w], ld_cluster4(in_cta(part0 + (w & ((1 << wph_log2) - 1)) * part_stride, w >> wph_log2)));
+            const float4* po = reinterpret_cast<const float4*>(p.parts + ((int64_t)b * p.H + h) * D + d);
+#pragma unroll 4
+            for (int k = sub; k < p.n_parts; k += share) add4(o, fast_exp2(pml[k * set + h].x - fw.top[gh]) * fw.inv[gh], po[k * set * (D / 4)]);
+        }
+        for (int m = 1; m < share; m <<= 1) {
+            o.x += __shfl_xor_sync(0xffffffffu, o.x, m);
+            o.y += __shfl_xor_sync(0xffffffffu, o.y, m);
+            o.z += __shfl_xor_sync(0xffffffffu, o.z, m);
+            o.w += __shfl_xor_sync(0xffffffffu, o.w, m);
+        }
+        if (h < 0 || sub) continue;
         const T* vn = (const T*)p.v_new + ((int64_t)b * p.Hkv + h / G) * D + d;
-        const float f = fw.fresh[gh];
-        float4 o = make_float4(f * to_f32<T>(vn[0]), f * to_f32<T>(vn[1]), f * to_f32<T>(vn[2]), f * to_f32<T>(vn[3]));
-        const uint32_t part0 = part + (slot << wph_log2) * part_stride + ((gh - slot * heads) * D + d) * 4;
-#pragma unroll 4
-        for (int w = 0; w < workers; ++w)
-            add4(o, weight[gh * workers + w], ld_cluster4(in_cta(part0 + (w & ((1 << wph_log2) - 1)) * part_stride, w >> wph_log2)));
-        const float4* po = reinterpret_cast<const float4*>(p.parts + ((int64_t)b * p.H + h) * D + d);
-#pragma unroll 4
-        for (int k = 0; k < p.n_parts; ++k) add4(o, fast_exp2(pml[k * set + h].x - fw.top[gh]) * fw.inv[gh], po[k * set * (D / 4)]);
+        add4(o, fw.fresh[gh], make_float4(to_f32<T>(vn[0]), to_f32<T>(vn[1]), to_f32<T>(vn[2]), to_f32<T>(vn[3])));
         T* out = (T*)p.out + ((int64_t)b * p.H + h) * D + d;
         out[0] = from_f32<T>(o.x);
         out[1] = from_f32<T>(o.y);
@@ -223,11 +235,12 @@ template <int D, bool E4> struct Ring {
     static constexpr int kStages = kStageBytes > 8192 ? 2 : 3;
     static constexpr int kWarpBytes = kStages * kStageBytes;
     static constexpr int kBytes = kWarps * kWarpBytes;
+    static constexpr int kCtasPerSm = 227 * 1024 / (kBytes + 4096) < 4 ? 227 * 1024 / (kBytes + 4096) : 4;
     static_assert(kWarpBytes >= 8 * D * 4, "a warp's partial result reuses its ring");
 };
 
 template <typename T, int D, bool E4>
-__global__ void __launch_bounds__(kWarps * 32, (227 * 1024 / (Ring<D, E4>::kBytes + 4096) < 4 ? 227 * 1024 / (Ring<D, E4>::kBytes + 4096) : 4))
+__global__ void __launch_bounds__(kWarps * 32, (Ring<D, E4>::kCtasPerSm))
 span_decode_kernel(const SpanParams p) {
     using R = Ring<D, E4>;
     using MT = typename std::conditional<E4, __half, T>::type;   // e4m3 rows are multiplied as fp16
@@ -469,10 +482,11 @@ span_decode_kernel(const SpanParams p) {
     }
     if (p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    cluster_sync();
+    if (p.splits > 1) cluster_sync();
+    else __syncthreads();
     fold<T, D>(p, s_fold, b, vh0, rank, (uint32_t)__cvta_generic_to_shared(ring_raw), R::kWarpBytes, (uint32_t)__cvta_generic_to_shared(s_ml),
                s_new, heads);
-    cluster_sync();              // nobody leaves while its shared memory is still read
+    if (p.splits > 1) cluster_sync();              // nobody leaves while its shared memory is still read
 }
 
 // Any head_dim up to 32 * DPL, any type: one cluster per (sequence, query head), a warp per token, a lane
@@ -584,16 +598,23 @@ int launch_mma(SpanParams p, int64_t span, cudaStream_t st) {
     const int G = p.H / p.Hkv;
     p.n_sets = (G + 7) / 8;
     const int vheads = p.Hkv * p.n_sets;
-    // Heads per CTA: four adjacent ones read 4 rows' worth of contiguous bytes per token; fewer (several
-    // warps per head) when the batch is too small to fill the machine that way even with 8 splits.
-    const int64_t slots = 148 * 2;
-    int hl = 2;
-    while (hl > 0 && ((1 << hl) > vheads || (int64_t)p.B * ((vheads + (1 << hl) - 1) >> hl) * 8 < slots)) --hl;
-    const int64_t units = (int64_t)p.B * ((vheads + (1 << hl) - 1) >> hl);
-    const int wph = kWarps >> hl;
-    const int64_t tiles = (span + kTile - 1) / kTile;
-    int s = 1;
-    while (s < 16 && units * s < slots && tiles > (int64_t)s * wph * 2) s *= 2;
+    // Heads per CTA and CTAs per sequence: one wave of CTAs, as full as a power of two makes it (a second wave
+    // costs a CTA's whole start and end, ~6 us; a cluster of 16 about 10 more).  Few heads per CTA (several warps to a head)
+    // start and end quickest: batch 8, 32 KV heads, 512 tokens 16.2 us with one head per CTA, 18.3 with four and
+    // clusters of four.  Four adjacent heads read 4 times the contiguous bytes per token, which counts once DRAM is
+    // the bound: batch 64, 8 KV heads, 4100 tokens 207 us with four heads and clusters of two, 258 with two, 356 with one.
+    const int64_t slots = 148 * Ring<D, E4>::kCtasPerSm, tiles = (span + kTile - 1) / kTile;
+    const int64_t bytes = (int64_t)p.B * span * 2 * p.Hkv * Ring<D, E4>::kRow;
+    auto units_of = [&](int hl) { return (int64_t)p.B * ((vheads + (1 << hl) - 1) >> hl); };
+    auto splits_of = [&](int hl) {
+        int s = 1;
+        while (s < 16 && units_of(hl) * s * 2 <= slots && tiles > (int64_t)s * (kWarps >> hl)) s *= 2;
+        return s;
+    };
+    int hl = 0;
+    while (hl < 2 && (2 << hl) <= vheads && (units_of(hl) > slots || (bytes > (100 << 20) && splits_of(hl + 1) <= 4))) ++hl;
+    const int64_t units = units_of(hl);
+    const int s = splits_of(hl);
     p.hpc_log2 = hl;
     p.splits = s;
     return launch(span_decode_kernel<T, D, E4>, p, units, Ring<D, E4>::kBytes, st, ready);

@@ -155,34 +155,78 @@ def rope_and_cache_write(Q, K, V, positions, cos, sin, slots, K_cache, V_cache, 
 # ----------------------------------------------------------------------------------------------
 # norm of every query and key head with the rotation (and the cache append) in one pass
 # ----------------------------------------------------------------------------------------------
-def _check_on(dev: torch.device, *tensors) -> None:
-    """``(tensor or None, name)`` pairs: CUDA tensors of one device (contiguity is the caller's business)."""
-    for x, name in tensors:
+def _check_on(names: str, *tensors) -> int:
+    """All tensors (None is skipped) are CUDA tensors of the first one's device, whose index is returned.
+    ``names``: theirs, separated by spaces, for the message."""
+    dev = -1
+    try:
+        dev = tensors[0].get_device()
+        for x in tensors:
+            if x is not None and (dev < 0 or x.get_device() != dev):
+                break
+        else:
+            return dev
+    except AttributeError:          # not a tensor
+        pass
+    for x, name in zip(tensors, names.split()):
         if x is None:
             continue
         if not isinstance(x, torch.Tensor) or not x.is_cuda:
             raise RuntimeError(f"{name} must be a CUDA tensor")
-        if x.device != dev:
-            raise RuntimeError(f"{name} must be on the same device as Q ({dev}), not on {x.device}")
+        if x.get_device() != dev:
+            raise RuntimeError(f"{name} must be on Q's device, not on {x.device}")
+    raise RuntimeError("Q must be a CUDA tensor")
+
+
+def _contiguous(x, name: str) -> None:
+    if not x.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
+
+
+def _table(x, name: str) -> None:
+    """A contiguous int32 tensor (its device has been checked)."""
+    if x.dtype != torch.int32:
+        raise RuntimeError(f"{name} must be int32 (expected scalar type Int but found {x.dtype})")
+    if not x.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
+
+
+class _on_index:
+    """`with torch.cuda.device(index)` that does nothing when it is already current."""
+    __slots__ = ("ctx",)
+
+    def __init__(self, index: int):
+        self.ctx = None if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            return self.ctx.__exit__(*exc)
+        return False
 
 
 def _flag_word(x) -> None:
-    if x is not None and (x.dtype != torch.int32 or x.numel() < 1):
+    if x.dtype != torch.int32 or x.numel() < 1:
         raise RuntimeError("err_flag must be an int32 tensor with one entry")
 
 
 def _rows(x, name: str) -> None:
-    """A matrix of whole rows: contiguous columns, rows any non-negative distance apart that keeps them disjoint."""
-    if x.dim() != 2 or (x.size(1) > 1 and x.stride(1) != 1) or (x.size(0) > 1 and x.stride(0) < x.size(1)):
+    """A matrix of whole rows: contiguous columns, rows any distance apart that keeps them disjoint."""
+    if x.dim() != 2 or not (x.is_contiguous() or ((x.size(1) <= 1 or x.stride(1) == 1) and
+                                                  (x.size(0) <= 1 or x.stride(0) >= x.size(1)))):
         raise RuntimeError(f"{name} must be two-dimensional with contiguous rows that do not overlap")
 
 
-def _kv_scales(kvd: int, k_scale, v_scale, hkv: int, dev) -> None:
+def _kv_scales(kvd: int, k_scale, v_scale, hkv: int, dev: int) -> None:
     if kvd != _lib.E4M3:
         return
     if k_scale is None or v_scale is None:
         raise RuntimeError("FP8 KV needs k_scale and v_scale (float32 [Hkv])")
-    _check_on(dev, (k_scale, "k_scale"), (v_scale, "v_scale"))
+    if _check_on("k_scale v_scale", k_scale, v_scale) != dev:
+        raise RuntimeError("k_scale and v_scale must be on Q's device")
     for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
         if t.dtype != torch.float32 or t.numel() != hkv or not t.is_contiguous():
             raise RuntimeError(f"{n} must be contiguous float32 [Hkv]")
@@ -209,73 +253,86 @@ def _may_overlap(a, b) -> bool:
 
 def _qk_norm_rope(what, Q, K, V, q_weight, k_weight, positions, cos, sin, slots, K_cache, V_cache, head_dim, eps,
                   k_scale, v_scale, out, err_flag):
-    _check_on(getattr(Q, "device", None), (Q, "Q"), (K, "K"), (V, "V"), (q_weight, "q_weight"), (k_weight, "k_weight"),
-              (positions, "positions"), (cos, "cos"), (sin, "sin"), (slots, "slots"), (K_cache, "K_cache"),
-              (V_cache, "V_cache"), (err_flag, "err_flag"))
-    _flag_word(err_flag)
-    dev, dt = Q.device, _dtype_code(Q, "Q")
-    for t, n in ((Q, "Q"), (K, "K")) + (((V, "V"),) if V is not None else ()):
-        _rows(t, n)
-        if t.dtype != Q.dtype or t.size(0) != Q.size(0):
-            raise RuntimeError("Q, K and V must share a dtype and the number of rows")
-    n_tokens = Q.size(0)
-    if head_dim <= 0 or Q.size(1) % head_dim or K.size(1) % head_dim or not Q.size(1) or not K.size(1):
+    dev = _check_on("Q K V q_weight k_weight positions cos sin slots K_cache V_cache err_flag", Q, K, V, q_weight, k_weight,
+                    positions, cos, sin, slots, K_cache, V_cache, err_flag)
+    if err_flag is not None:
+        _flag_word(err_flag)
+    dtype = Q.dtype
+    dt = _dtype_code(Q, "Q")
+    _rows(Q, "Q")
+    _rows(K, "K")
+    n_tokens, q_cols = Q.shape
+    k_rows, k_cols = K.shape
+    if K.dtype != dtype or k_rows != n_tokens:
+        raise RuntimeError("Q, K and V must share a dtype and the number of rows")
+    if head_dim <= 0 or q_cols % head_dim or k_cols % head_dim or not q_cols or not k_cols:
         raise RuntimeError("Q.size(1) and K.size(1) must be positive multiples of head_dim")
-    _int32(positions, "positions")
+    _table(positions, "positions")
     if positions.numel() != n_tokens:
         raise RuntimeError("positions must have one entry per row of Q")
-    for t, n in ((cos, "cos"), (sin, "sin"), (q_weight, "q_weight"), (k_weight, "k_weight")):
-        _check_input(t, n)
-    if cos.dim() != 2 or sin.shape != cos.shape or 2 * cos.size(1) > head_dim:
+    if not (cos.is_contiguous() and sin.is_contiguous() and q_weight.is_contiguous() and k_weight.is_contiguous()):
+        raise RuntimeError("cos, sin, q_weight and k_weight must be contiguous")
+    cos_shape = cos.shape
+    if len(cos_shape) != 2 or sin.shape != cos_shape or 2 * cos_shape[1] > head_dim:
         raise RuntimeError("cos and sin must be [max_pos, rot_half] with 2 * rot_half <= head_dim")
     if q_weight.numel() != head_dim or k_weight.numel() != head_dim:
         raise RuntimeError("q_weight and k_weight must have head_dim entries")
-    if cos.dtype != sin.dtype or cos.dtype not in (Q.dtype, torch.float32):
+    t_dtype, w_dtype = cos.dtype, q_weight.dtype
+    if sin.dtype != t_dtype or (t_dtype != dtype and t_dtype != torch.float32):
         raise RuntimeError("cos and sin must both have Q's dtype or both be float32")
-    if q_weight.dtype != k_weight.dtype or q_weight.dtype not in (Q.dtype, torch.float32):
+    if k_weight.dtype != w_dtype or (w_dtype != dtype and w_dtype != torch.float32):
         raise RuntimeError("q_weight and k_weight must both have Q's dtype or both be float32")
     if not eps >= 0:
         raise RuntimeError("eps must not be negative")
-    hk, kvd, n_slots = K.size(1) // head_dim, dt, 0
+    hk, kvd, n_slots, v_stride = k_cols // head_dim, dt, 0, 0
     if slots is not None:
-        _int32(slots, "slots")
+        _table(slots, "slots")
         if slots.numel() != n_tokens:
             raise RuntimeError("slots must have one entry per row of Q")
-        _check_input(K_cache, "K_cache")
-        _check_input(V_cache, "V_cache")
-        kvd, n_slots = _kv_code(K_cache, Q), K_cache.size(0)
-        if V.shape != K.shape or K_cache.dim() != 2 or K_cache.size(1) != K.size(1) or V_cache.shape != K_cache.shape:
+        _rows(V, "V")
+        _contiguous(K_cache, "K_cache")
+        _contiguous(V_cache, "V_cache")
+        kvd, shape = _kv_code(K_cache, Q), K_cache.shape
+        if V.dtype != dtype or V.shape != K.shape or len(shape) != 2 or shape[1] != k_cols or V_cache.shape != shape:
             raise RuntimeError("V must match K, and the pools must be [slots, Hk*head_dim]")
         if V_cache.dtype != K_cache.dtype:
             raise RuntimeError("K_cache and V_cache must share a dtype")
         _kv_scales(kvd, k_scale, v_scale, hk, dev)
+        n_slots, v_stride = shape[0], V.stride(0)
     if out is None:
         # contiguous whatever the inputs' strides are: what the attention operators take
-        Qo = torch.empty(n_tokens, Q.size(1), dtype=Q.dtype, device=dev)
-        Ko = torch.empty(n_tokens, K.size(1), dtype=Q.dtype, device=dev)
+        Qo = torch.empty_like(Q, memory_format=torch.contiguous_format)
+        Ko = torch.empty_like(K, memory_format=torch.contiguous_format)
+        qo_stride, ko_stride = q_cols, k_cols
     else:
         Qo, Ko = out
-        _check_on(dev, (Qo, "out[0]"), (Ko, "out[1]"))
-        for t, x, n in ((Qo, Q, "out[0]"), (Ko, K, "out[1]")):
-            _rows(t, n)
-            if t.shape != x.shape or t.dtype != x.dtype:
-                raise RuntimeError(f"{n} must have the shape and dtype of its input")
-            for y in (Q, K, V):
-                same = y is x and t.data_ptr() == x.data_ptr() and (t.stride(0) == x.stride(0) or n_tokens <= 1)
-                if y is not None and not same and _may_overlap(t, y):
-                    raise RuntimeError(f"{n} must be its input itself or share no memory with Q, K and V")
-        if _may_overlap(Qo, Ko):
-            raise RuntimeError("out[0] and out[1] must not share memory")
+        _check_norm_out(Qo, Ko, Q, K, V)
+        qo_stride, ko_stride = Qo.stride(0), Ko.stride(0)
     if n_tokens == 0:
         return Qo, Ko
-    with _on_device(dev):
+    with _on_index(dev):
         check(lib.attn_b200_qk_norm_rope(
-            Q.data_ptr(), K.data_ptr(), _ptr(V), Qo.data_ptr(), Ko.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
-            positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ptr(slots), _ptr(K_cache), _ptr(V_cache), n_tokens,
-            Q.size(1) // head_dim, hk, head_dim, cos.size(1), cos.size(0), n_slots, Q.stride(0), K.stride(0),
-            0 if V is None else V.stride(0), Qo.stride(0), Ko.stride(0), eps, dt, _DT[q_weight.dtype], _DT[cos.dtype], kvd,
-            _ptr(k_scale), _ptr(v_scale), _ptr(err_flag), _stream()), what)
+            Q.data_ptr(), K.data_ptr(), None if V is None else V.data_ptr(), Qo.data_ptr(), Ko.data_ptr(), q_weight.data_ptr(),
+            k_weight.data_ptr(), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ptr(slots), _ptr(K_cache), _ptr(V_cache),
+            n_tokens, q_cols // head_dim, hk, head_dim, cos_shape[1], cos_shape[0], n_slots, Q.stride(0), K.stride(0), v_stride,
+            qo_stride, ko_stride, eps, dt, _DT[w_dtype], _DT[t_dtype], kvd, _ptr(k_scale), _ptr(v_scale), _ptr(err_flag),
+            _stream()), what)
     return Qo, Ko
+
+
+def _check_norm_out(Qo, Ko, Q, K, V) -> None:
+    if _check_on("Q out[0] out[1]", Q, Qo, Ko) < 0:
+        raise RuntimeError("out must be CUDA tensors")
+    for t, x, n in ((Qo, Q, "out[0]"), (Ko, K, "out[1]")):
+        _rows(t, n)
+        if t.shape != x.shape or t.dtype != x.dtype:
+            raise RuntimeError(f"{n} must have the shape and dtype of its input")
+        for y in (Q, K, V):
+            same = y is x and t.data_ptr() == x.data_ptr() and (t.stride(0) == x.stride(0) or x.size(0) <= 1)
+            if y is not None and not same and _may_overlap(t, y):
+                raise RuntimeError(f"{n} must be its input itself or share no memory with Q, K and V")
+    if _may_overlap(Qo, Ko):
+        raise RuntimeError("out[0] and out[1] must not share memory")
 
 
 def qk_norm_rope(Q, K, q_weight, k_weight, positions, cos, sin, head_dim: int, *, eps: float = 1e-6, out=None,
@@ -801,38 +858,36 @@ def lse_combine(parts, Q, K=None, V=None, *, num_heads: int, scale: Optional[flo
 # ----------------------------------------------------------------------------------------------
 # sliding window with sink tokens, shared prefix
 # ----------------------------------------------------------------------------------------------
-_INT_MAX = 0x7fffffff
-
-
-def _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_scale):
-    """Checks what the single-token operators share; returns (B, D, Hkv, Q's dtype code, the pools')."""
-    for t, n in ((Q, "Q"), (K, "K"), (V, "V"), (K_cache, "K_cache"), (V_cache, "V_cache")):
-        _check_input(t, n)
-        if t.dim() != 2:
-            raise RuntimeError(f"{n} must be two-dimensional")
+def _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_scale, dev):
+    """Checks what the single-token operators share (devices are checked); returns (B, D, Hkv, Q's dtype code, the pools')."""
+    if not (Q.is_contiguous() and K.is_contiguous() and V.is_contiguous() and K_cache.is_contiguous() and V_cache.is_contiguous()):
+        for t, n in ((Q, "Q"), (K, "K"), (V, "V"), (K_cache, "K_cache"), (V_cache, "V_cache")):
+            _contiguous(t, n)
+    dtype, pool_dtype, q_shape, k_shape, shape = Q.dtype, K_cache.dtype, Q.shape, K.shape, K_cache.shape
+    if len(q_shape) != 2 or len(shape) != 2:
+        raise RuntimeError("Q and the pools must be two-dimensional")
     qd, kvd = _dtype_code(Q, "Q"), _kv_code(K_cache, Q)
-    if V_cache.dtype != K_cache.dtype or K.dtype != Q.dtype or V.dtype != Q.dtype:
+    if V_cache.dtype != pool_dtype or K.dtype != dtype or V.dtype != dtype:
         raise RuntimeError("dtype mismatch between Q/K/V or K_cache/V_cache")
-    B, dim = Q.shape
+    B, dim = q_shape
     if num_heads <= 0 or dim % num_heads or not dim:
         raise RuntimeError("Q.size(1) must be a positive multiple of num_heads")
-    D = dim // num_heads
-    cols = K_cache.size(1)
-    if not cols or cols % D or num_heads % (cols // D) or V_cache.shape != K_cache.shape:
+    D, cols = dim // num_heads, shape[1]
+    if not cols or cols % D or num_heads % (cols // D) or V_cache.shape != shape:
         raise RuntimeError("K_cache/V_cache must be [slots, Hkv*D] with Hkv dividing num_heads")
-    if K.shape != (B, cols) or V.shape != (B, cols):
+    if k_shape != (B, cols) or V.shape != k_shape:
         raise RuntimeError("K and V must be [B, Hkv*D] like the pools' rows")
-    _int32(offsets, "offsets")
+    _table(offsets, "offsets")
     if offsets.numel() != B:
         raise RuntimeError("offsets must have one entry per sequence")
-    _kv_scales(kvd, k_scale, v_scale, cols // D, Q.device)
+    _kv_scales(kvd, k_scale, v_scale, cols // D, dev)
     return B, D, cols // D, qd, kvd
 
 
 def _output(out, Q):
     if out is None:
         return torch.empty_like(Q)
-    _check_input(out, "out")
+    _contiguous(out, "out")
     if out.shape != Q.shape or out.dtype != Q.dtype:
         raise RuntimeError("out must have Q's shape and dtype")
     return out
@@ -841,7 +896,7 @@ def _output(out, Q):
 def _window_args(window, n_sinks):
     if int(window) != window or window < 1 or int(n_sinks) != n_sinks or n_sinks < 0:
         raise RuntimeError("window must be a positive and n_sinks a non-negative whole number")
-    return min(int(window), _INT_MAX), min(int(n_sinks), _INT_MAX)
+    return min(int(window), 0x7fffffff), min(int(n_sinks), 0x7fffffff)
 
 
 def paged_window_attention_forward(Q, K, V, K_cache, V_cache, cache_indices, offsets, num_heads: int, window: int,
@@ -858,12 +913,13 @@ def paged_window_attention_forward(Q, K, V, K_cache, V_cache, cache_indices, off
     outside the pools is skipped and sets its bit in ``err_flag``.  One kernel, no workspace.  Returns
     O ``[B, H*D]``.
     """
-    _check_on(getattr(Q, "device", None), (Q, "Q"), (K, "K"), (V, "V"), (K_cache, "K_cache"), (V_cache, "V_cache"),
-              (cache_indices, "cache_indices"), (offsets, "offsets"), (out, "out"), (err_flag, "err_flag"))
-    _flag_word(err_flag)
-    B, D, Hkv, qd, kvd = _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_scale)
+    dev = _check_on("Q K V K_cache V_cache cache_indices offsets out err_flag", Q, K, V, K_cache, V_cache, cache_indices, offsets,
+                    out, err_flag)
+    if err_flag is not None:
+        _flag_word(err_flag)
+    B, D, Hkv, qd, kvd = _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_scale, dev)
     window, n_sinks = _window_args(window, n_sinks)
-    _int32(cache_indices, "cache_indices")
+    _table(cache_indices, "cache_indices")
     max_blocks = 0
     if block_size != 1:
         if block_size < 1 or cache_indices.dim() != 2 or cache_indices.size(0) != B:
@@ -872,7 +928,7 @@ def paged_window_attention_forward(Q, K, V, K_cache, V_cache, cache_indices, off
     O = _output(out, Q)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    with _on_device(Q.device):
+    with _on_index(dev):
         check(lib.attn_b200_paged_window_decode(
             Q.data_ptr(), K.data_ptr(), V.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), cache_indices.data_ptr(),
             offsets.data_ptr(), O.data_ptr(), B, num_heads, Hkv, D, cache_indices.numel(), K_cache.size(0), block_size,
@@ -897,15 +953,16 @@ def paged_window_prefill_attention(Q, K_cache, V_cache, cache_indices, kv_offset
     cores, where a non-finite value in V also reaches the queries of the same 128-row tile that do not see it;
     every other type and head_dim up to 512 runs the generic kernel.  Returns O ``[sum q_len, H*D]``.
     """
-    _check_on(getattr(Q, "device", None), (Q, "Q"), (K_cache, "K_cache"), (V_cache, "V_cache"), (cache_indices, "cache_indices"),
-              (kv_offsets, "kv_offsets"), (q_offsets, "q_offsets"), (out, "out"), (err_flag, "err_flag"))
-    _flag_word(err_flag)
+    dev = _check_on("Q K_cache V_cache cache_indices kv_offsets q_offsets out err_flag", Q, K_cache, V_cache, cache_indices, kv_offsets,
+                    q_offsets, out, err_flag)
+    if err_flag is not None:
+        _flag_word(err_flag)
     for t, n in ((Q, "Q"), (K_cache, "K_cache"), (V_cache, "V_cache")):
-        _check_input(t, n)
+        _contiguous(t, n)
         if t.dim() != 2:
             raise RuntimeError(f"{n} must be two-dimensional")
     for t, n in ((cache_indices, "cache_indices"), (kv_offsets, "kv_offsets"), (q_offsets, "q_offsets")):
-        _int32(t, n)
+        _table(t, n)
     dt = _dtype_code(Q, "Q")
     if K_cache.dtype != Q.dtype or V_cache.dtype != Q.dtype or V_cache.shape != K_cache.shape:
         raise RuntimeError("K_cache and V_cache must share Q's dtype and each other's shape")
@@ -919,7 +976,7 @@ def paged_window_prefill_attention(Q, K_cache, V_cache, cache_indices, kv_offset
     O = _output(out, Q)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    with _on_device(Q.device):
+    with _on_index(dev):
         if max_q_len is None:
             max_q_len = max(0, int(torch.diff(q_offsets, prepend=q_offsets.new_zeros(1)).max().item())) if B else 0
         check(lib.attn_b200_paged_window_prefill(
@@ -951,13 +1008,13 @@ def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, c
     ``shared_prefix_workspace_bytes(...)``) holds nothing between calls; two calls that may overlap need one each.
     A slot outside the pools is skipped and sets its bit in ``err_flag``.  Returns O ``[B, H*D]``.
     """
-    _check_on(getattr(Q, "device", None), (Q, "Q"), (K, "K"), (V, "V"), (K_cache, "K_cache"), (V_cache, "V_cache"),
-              (prefix_indices, "prefix_indices"), (cache_indices, "cache_indices"), (offsets, "offsets"), (workspace, "workspace"),
-              (out, "out"), (err_flag, "err_flag"))
-    _flag_word(err_flag)
-    B, D, Hkv, qd, kvd = _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_scale)
-    _int32(prefix_indices, "prefix_indices")
-    _int32(cache_indices, "cache_indices")
+    dev = _check_on("Q K V K_cache V_cache prefix_indices cache_indices offsets workspace out err_flag", Q, K, V, K_cache, V_cache,
+                    prefix_indices, cache_indices, offsets, workspace, out, err_flag)
+    if err_flag is not None:
+        _flag_word(err_flag)
+    B, D, Hkv, qd, kvd = _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_scale, dev)
+    _table(prefix_indices, "prefix_indices")
+    _table(cache_indices, "cache_indices")
     O = _output(out, Q)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
@@ -968,7 +1025,7 @@ def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, c
             workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
     elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
         raise RuntimeError(f"workspace too small: {need} contiguous bytes needed")
-    with _on_device(Q.device):
+    with _on_index(dev):
         check(lib.attn_b200_shared_prefix_decode(
             Q.data_ptr(), K.data_ptr(), V.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), prefix_indices.data_ptr(),
             cache_indices.data_ptr(), offsets.data_ptr(), O.data_ptr(), _ptr(workspace), need, B, num_heads, Hkv, D, P,
