@@ -61,7 +61,7 @@ template <int HD> struct Smem {
     alignas(1024) unsigned char q[2][kTile];
     alignas(1024) unsigned char k[kStages][kTile];
     alignas(1024) unsigned char v[kStages][kTile];
-    alignas(1024) unsigned char extra[2][kTile / 2];    // window: output staging; e4m3: raw K tile, raw V tile
+    alignas(1024) unsigned char extra[2][kSub];         // window: output staging; e4m3: raw K tile, raw V tile
     alignas(16) unsigned char bad[4][BN];               // rows of a tile without a pool row (ring of four tiles)
     signed char row_exp[2][BM];                         // bf16 queries over e4m3 rows: the power of two taken out of q
     Item item[kItems];
@@ -179,7 +179,7 @@ __device__ __forceinline__ void prefix_item(const AttendParams& p, Item& it) {
 // over S, keeps the reference maximum m and the denominator l.  Visible entries u of the list: u <= hi and
 // (u >= lo or u < ns).  `c0`: tiles this warpgroup has seen before (barrier phases), `g0`: tiles of the CTA
 // before this item.  Returns false when a wait ran out.
-template <typename MT, int HD, int kPolyOf8>
+template <typename MT, int HD>
 __device__ __forceinline__ bool softmax_rows(Smem<HD>& sm, int w, uint32_t s_addr, uint32_t o_addr, int w0, int j0, int step,
                                              int count, int c0, int g0, int hi, int lo, int ns, float scale, float& m_ref, float& l) {
     AbortBox* const wc = &sm.box;
@@ -241,14 +241,12 @@ __device__ __forceinline__ bool softmax_rows(Smem<HD>& sm, int w, uint32_t s_add
                     float x0, x1, x2, x3, p0, p1, p2, p3;
                     fma2(x0, x1, sv[c * 64 + e], sv[c * 64 + e + 1], scale, scale, nm, nm);
                     fma2(x2, x3, sv[c * 64 + e + 2], sv[c * 64 + e + 3], scale, scale, nm, nm);
+                    // all on the special-function unit: with two of eight as a cubic on the FMA pipe, which the packed
+                    // prefill gains from, four prompts took 403 us instead of 380 (issue slots, not the unit, are short here)
                     p0 = fast_exp2(x0);
                     p1 = fast_exp2(x1);
-                    if (kPolyOf8 == 2 && (e & 4)) {
-                        exp2_poly2(p2, p3, x2, x3);
-                    } else {
-                        p2 = fast_exp2(x2);
-                        p3 = fast_exp2(x3);
-                    }
+                    p2 = fast_exp2(x2);
+                    p3 = fast_exp2(x3);
                     add2(rs4[0], rs4[1], rs4[0], rs4[1], p0, p1);
                     add2(rs4[2], rs4[3], rs4[2], rs4[3], p2, p3);
                     pk[e >> 1] = pack2<MT>(p0, p1);
@@ -361,7 +359,7 @@ enum Mode { kWindow, kPrefixPair, kPrefixSplit };      // kPrefixSplit: AttendPa
 template <typename T, int HD, int kMode, bool E4>
 __global__ void __launch_bounds__(kThreads, 1)
 attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                 const __grid_constant__ CUtensorMap map_v, const AttendParams p) {
+                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o, const AttendParams p) {
     constexpr bool kPrefix = kMode != kWindow, key_split = kMode == kPrefixSplit;
     using MT = typename std::conditional<E4, __half, T>::type;       // e4m3 rows are multiplied as fp16
     using R = Cfg<E4>;
@@ -682,7 +680,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 // W: the warpgroup, a compile-time 0 or 1, so that all of this stays in registers
                 auto start_tile = [&](auto W, int t, int wide) -> bool {                  // Q.K of tile t (of the CTA)
                     constexpr int w = decltype(W)::value;
-                    if (!mbar_wait_spin(&sm.k_full[t & 1], (t >> 1) & 1, wc)) return false;
+                    if (!mbar_wait(&sm.k_full[t & 1], (t >> 1) & 1, wc)) return false;
                     tc_fence_after();
                     const uint64_t a = qd + (w ? (key_split ? 0 : kTile16) : 0), b2 = kd + (t & 1) * kTile16;
                     const uint32_t idesc = idesc0 | ((uint32_t)(wide >> 3) << 17);
@@ -701,19 +699,19 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     ++done;
                     const uint64_t v = vd + (t & 1) * kTile16;
                     const uint32_t d = tmem + 256 + w * 128, a = tmem + w * 128;
-                    if (first && (w ? uses1 : uses0) > 0 && !mbar_wait_spin(&sm.o_free[w], ((w ? uses1 : uses0) - 1) & 1, wc)) return false;
-                    if (!mbar_wait_spin(&sm.p_half[w], ph, wc)) return false;
-                    if (!mbar_wait_spin(&sm.v_full[t & 1], (t >> 1) & 1, wc)) return false;
+                    if (first && (w ? uses1 : uses0) > 0 && !mbar_wait(&sm.o_free[w], ((w ? uses1 : uses0) - 1) & 1, wc)) return false;
+                    if (!mbar_wait(&sm.p_half[w], ph, wc)) return false;
+                    if (!mbar_wait(&sm.v_full[t & 1], (t >> 1) & 1, wc)) return false;
                     tc_fence_after();
                     if (wide == BN) {
 #pragma unroll
                         for (int kk = 0; kk < BN / 32; ++kk) umma_f16_ts(d, a + kk * 8, v + ((kk * 2048) >> 4), idesc_pv, (!first || kk > 0) ? 1u : 0u);
-                        if (!mbar_wait_spin(&sm.p_full[w], ph, wc)) return false;
+                        if (!mbar_wait(&sm.p_full[w], ph, wc)) return false;
                         tc_fence_after();
 #pragma unroll
                         for (int kk = BN / 32; kk < BN / 16; ++kk) umma_f16_ts(d, a + kk * 8, v + ((kk * 2048) >> 4), idesc_pv, 1u);
                     } else {
-                        if (!mbar_wait_spin(&sm.p_full[w], ph, wc)) return false;
+                        if (!mbar_wait(&sm.p_full[w], ph, wc)) return false;
                         tc_fence_after();
 #pragma unroll 1
                         for (int kk = 0; kk < wide / 16; ++kk)
@@ -731,7 +729,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     // columns that a tile is multiplied in: whole, or its keys rounded up to 32
                     const int wide0 = ip->w0 > 96 ? BN : (ip->w0 + 31) / 32 * 32;
                     auto wide = [&](int j) { return j ? BN : wide0; };
-                    bool ok = mbar_wait_spin(&sm.q_full[0], uses0 & 1, wc);        // the first query tile always has rows
+                    bool ok = mbar_wait(&sm.q_full[0], uses0 & 1, wc);        // the first query tile always has rows
                     if (key_split) {
                         if (ok) ok = start_tile(W0, 0, wide0);
                         umma_commit(&sm.k_empty[0]);
@@ -755,7 +753,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                             }
                         }
                     } else {
-                        if (ok && je1 > jb1) ok = mbar_wait_spin(&sm.q_full[1], uses1 & 1, wc);
+                        if (ok && je1 > jb1) ok = mbar_wait(&sm.q_full[1], uses1 & 1, wc);
                         // every tile is some warpgroup's: the list is the union of two overlapping stretches
                         if (ok && jb0 == 0) ok = start_tile(W0, g, wide0);
                         if (ok && je0 == 1) umma_commit(&sm.q_empty[0]);
@@ -851,8 +849,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     scale *= __int_as_float((127 + sm.row_exp[key_split ? 0 : w][r]) << 23);
                 }
             }
-            // fp16: every exponential on the special-function unit; bf16: two of eight as a cubic on the FMA pipe
-            if (count > 0 && !__all_sync(0xffffffffu, softmax_rows<MT, HD, std::is_same<MT, __nv_bfloat16>::value ? 2 : 0>(
+            if (count > 0 && !__all_sync(0xffffffffu, softmax_rows<MT, HD>(
                                                           sm, w, s_addr, o_addr, it.w0, it.jb[w], step, count, c0, g, hi, lo, ns, scale, m, l)))
                 break;
             c0 += count;
@@ -906,33 +903,48 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 mbar_arrive(&sm.o_free[w]);         // the next item may overwrite the accumulator
                 // a row none of whose keys has a pool row is zero
                 const float inv = m > -INFINITY || l != l ? 1.f / l : 0.f;
-                constexpr int kPass = kTileBytes / 2 / BM / 2;              // columns per pass: half a row
-                const uint32_t buf = smem_u32(sm.extra[w]) + (warp & 3) * (kTileBytes / 8);
+                // A warp's 4 KB of staging hold 64 columns of its 32 rows in the 128-byte-swizzled layout of a TMA box; one
+                // lane stores the box, or, where the chunk ends inside it, the lanes copy the rows that exist.
+                unsigned char* const stage = sm.extra[w] + (warp & 3) * 4096;
+                const bool box = row_w + 32 <= it.n_rows;
 #pragma unroll
-                for (int c = 0; c < HD; c += kPass) {
+                for (int c = 0; c < HD; c += 64) {
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");     // the store before has read it
+                    __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < kPass / 8; ++e) {
+                    for (int e = 0; e < 8; ++e) {
                         const float* o8 = ov + c + e * 8;
-                        st_shared16(buf + lr * (kPass * 2) + ((e ^ (lr & (kPass / 8 - 1))) << 4), pack2<T>(o8[0] * inv, o8[1] * inv),
+                        st_shared16(smem_u32(stage) + lr * 128 + ((e ^ (lr & 7)) << 4), pack2<T>(o8[0] * inv, o8[1] * inv),
                                     pack2<T>(o8[2] * inv, o8[3] * inv), pack2<T>(o8[4] * inv, o8[5] * inv), pack2<T>(o8[6] * inv, o8[7] * inv));
                     }
-                    __syncwarp();
-                    constexpr int kLanes = kPass / 8, kRows = 32 / kLanes;
-                    Rows rows = rows_from(it, w, row_w + lane / kLanes);
-                    T* const dst = (T*)p.out + c + lane % kLanes * 8;
-#pragma unroll
-                    for (int i = 0; i < 32; i += kRows) {
-                        const int rr = i + lane / kLanes, cc = lane % kLanes;
-                        const uint4 x = ld_shared16(buf + rr * (kPass * 2) + ((cc ^ (rr & (kLanes - 1))) << 4));
-                        const int64_t at = rows.at();
-                        if (at >= 0) *reinterpret_cast<uint4*>(dst + at) = x;
-                        rows.next(kRows);
+                    if (box) {
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) {
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+                                         ::"l"(reinterpret_cast<uint64_t>(&map_o)), "r"(it.head[w] * HD + c), "r"((int)(it.q_beg + row_w)),
+                                           "r"(smem_u32(stage)) : "memory");
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        }
+                    } else {
+                        __syncwarp();
+                        Rows rows = rows_from(it, w, row_w + lane / 8);
+                        T* const dst = (T*)p.out + c + lane % 8 * 8;
+#pragma unroll 1
+                        for (int i = 0; i < 32; i += 4) {
+                            const int rr = i + lane / 8, cc = lane % 8;
+                            const uint4 x = ld_shared16(smem_u32(stage) + rr * 128 + ((cc ^ (rr & 7)) << 4));
+                            const int64_t at = rows.at();
+                            if (at >= 0) *reinterpret_cast<uint4*>(dst + at) = x;
+                            rows.next(4);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
             }
             done_with(n);
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // shared memory stays until the stores have read it
     }
     tc_fence_before();
     __syncthreads();
@@ -1025,18 +1037,20 @@ int launch(const AttendParams& p, dim3 grid, cudaStream_t st) {
             return (int)e;
         ready.fetch_or(1ull << dev, std::memory_order_release);
     }
-    CUtensorMap mq, mk, mv;
+    CUtensorMap mq, mk, mv, mo;
     const int64_t cols = (int64_t)p.Hkv * HD;
     int rc;
     if ((rc = make_map(&mk, p.k_cache, p.n_slots, cols, E4 ? 1 : 2, E4 ? HD : 64, 1, !E4)) ||
         (rc = make_map(&mv, p.v_cache, p.n_slots, cols, E4 ? 1 : 2, E4 ? HD : 64, 1, !E4)))
         return rc;
     if (kMode == kWindow) {
-        if ((rc = make_map(&mq, p.q, p.n_q_tokens, (int64_t)p.H * HD, 2, 64, BM, true))) return rc;
+        if ((rc = make_map(&mq, p.q, p.n_q_tokens, (int64_t)p.H * HD, 2, 64, BM, true)) ||
+            (rc = make_map(&mo, p.out, p.n_q_tokens, (int64_t)p.H * HD, 2, 64, 32, true)))
+            return rc;
     } else {
-        mq = mk;               // not used
+        mq = mo = mk;          // not used
     }
-    return launch_dependent(attend_tc_kernel<T, HD, kMode, E4>, grid, kThreads, smem, st, mq, mk, mv, p);
+    return launch_dependent(attend_tc_kernel<T, HD, kMode, E4>, grid, kThreads, smem, st, mq, mk, mv, mo, p);
 }
 
 }  // namespace

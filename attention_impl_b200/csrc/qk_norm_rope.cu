@@ -94,10 +94,10 @@ __device__ __forceinline__ uint32_t e4m3x4(const float* f) {
 template <typename T> __device__ __forceinline__ void store_pool(void* pool, int64_t at, const float* f, const float* scale, int head) {
     if (scale) {
         if constexpr (Vec<T>::N == 8) {
-            const float s = scale[head];
+            const float r = fminf(1.f / scale[head], 3e38f);          // x / scale to 2 units in the last place, 0 stays 0
             float g[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] = f[i] / s;
+            for (int i = 0; i < 8; ++i) g[i] = f[i] * r;
             *reinterpret_cast<uint2*>((char*)pool + at) = make_uint2(e4m3x4(g), e4m3x4(g + 4));
         }
     } else {

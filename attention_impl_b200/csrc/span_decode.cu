@@ -208,7 +208,7 @@ __device__ __forceinline__ void fold(const SpanParams& p, FoldWeights& fw, int b
             for (int w = sub; w < workers; w += share)
                 add4(o, weight[gh * workers + w], ld_cluster4(in_cta(part0 + (w & ((1 << wph_log2) - 1)) * part_stride, w >> wph_log2)));
             const float4* po = reinterpret_cast<const float4*>(p.parts + ((int64_t)b * p.H + h) * D + d);
-#pragma unroll 4
+#pragma unroll 12
             for (int k = sub; k < p.n_parts; k += share) add4(o, fast_exp2(pml[k * set + h].x - fw.top[gh]) * fw.inv[gh], po[k * set * (D / 4)]);
         }
         for (int m = 1; m < share; m <<= 1) {
