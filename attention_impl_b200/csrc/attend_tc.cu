@@ -32,7 +32,6 @@ using namespace tc;
 
 constexpr int BM = 128, BN = 128;
 constexpr int kSub = 128 * 128;                 // bytes of a [128 rows x 64 elements] 128-byte-swizzled sub-tile
-constexpr int kStages = 2;
 constexpr int kItems = 4;                       // items published ahead
 // Warps 0-3 and 4-7 softmax, 8 item list, 9 MMA thread, 10 query tiles; 12-15 K and V, 32 rows of a tile each.  With
 // e4m3 rows 12-13 and 14-15 turn the raw K and V rows into fp16.
@@ -56,13 +55,18 @@ struct Item {
     int part;                  // prefix: first of this CTA's partial sets
 };
 
-template <int HD> struct Smem {
+enum Mode { kWindow, kPrefixPair, kPrefixSplit };      // kPrefixSplit: AttendParams::key_split
+
+template <int HD, int kMode, bool E4> struct Smem {
     static constexpr int kTile = HD / 64 * kSub;
-    alignas(1024) unsigned char q[2][kTile];
+    // Two stages each of K and V, three where one query tile leaves room: a batch that fits one tile waits for DRAM
+    static constexpr int kStages = kMode == kPrefixSplit && !E4 ? 3 : 2;
+    static constexpr int kExtra = kMode == kWindow || E4 ? kSub : 16;
+    alignas(1024) unsigned char q[kMode == kPrefixSplit ? 1 : 2][kTile];
     alignas(1024) unsigned char k[kStages][kTile];
     alignas(1024) unsigned char v[kStages][kTile];
-    alignas(1024) unsigned char extra[2][kSub];         // window: output staging; e4m3: raw K tile, raw V tile
-    alignas(16) unsigned char bad[4][BN];               // rows of a tile without a pool row (ring of four tiles)
+    alignas(1024) unsigned char extra[2][kExtra];       // window: output staging; e4m3: raw K tile, raw V tile
+    uint32_t bad[8][4];                                 // bit r: row r of a tile has no pool row (ring of eight tiles)
     signed char row_exp[2][BM];                         // bf16 queries over e4m3 rows: the power of two taken out of q
     Item item[kItems];
     alignas(8) unsigned long long item_full[kItems], item_empty[kItems];
@@ -179,8 +183,8 @@ __device__ __forceinline__ void prefix_item(const AttendParams& p, Item& it) {
 // over S, keeps the reference maximum m and the denominator l.  Visible entries u of the list: u <= hi and
 // (u >= lo or u < ns).  `c0`: tiles this warpgroup has seen before (barrier phases), `g0`: tiles of the CTA
 // before this item.  Returns false when a wait ran out.
-template <typename MT, int HD>
-__device__ __forceinline__ bool softmax_rows(Smem<HD>& sm, int w, uint32_t s_addr, uint32_t o_addr, int w0, int j0, int step,
+template <typename MT, int HD, typename SM>
+__device__ __forceinline__ bool softmax_rows(SM& sm, int w, uint32_t s_addr, uint32_t o_addr, int w0, int j0, int step,
                                              int count, int c0, int g0, int hi, int lo, int ns, float scale, float& m_ref, float& l) {
     AbortBox* const wc = &sm.box;
     constexpr float kLazy = 8.f;          // P <= 2^8: O is rescaled rarely
@@ -215,7 +219,7 @@ __device__ __forceinline__ bool softmax_rows(Smem<HD>& sm, int w, uint32_t s_add
         if (!mbar_wait(&sm.s_full[w], (c0 + i) & 1, wc)) return false;
         tc_fence_after();
         const bool any_bad = *(volatile int*)&sm.any_bad;
-        const unsigned char* const bad = sm.bad[(g0 + j) & 3];
+        const uint32_t* const bad = sm.bad[(g0 + j) & 7];
         const int h = min(hi - base, keys - 1), lw = lo - base, s = ns - base;     // in columns of this tile
         if (keys == BN && !__any_sync(0xffffffffu, any_bad || h < BN - 1 || (lw > 0 && s < BN))) {
             float sv[BN];
@@ -273,11 +277,7 @@ __device__ __forceinline__ bool softmax_rows(Smem<HD>& sm, int w, uint32_t s_add
             auto bits = [&](int c) -> uint32_t {
                 auto below = [&](int x) { return x <= c ? 0u : x >= c + 32 ? 0xffffffffu : (1u << (x - c)) - 1u; };     // columns < x
                 uint32_t m = below(h + 1) & (~below(lw) | below(s));
-                if (any_bad) {
-                    const uint32_t* b4 = reinterpret_cast<const uint32_t*>(bad + c);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) m &= ~(((b4[e] & 1u) | (b4[e] >> 7 & 2u) | (b4[e] >> 14 & 4u) | (b4[e] >> 21 & 8u)) << (4 * e));
-                }
+                if (any_bad) m &= ~bad[c >> 5];
                 return m;
             };
             float mx = -INFINITY;
@@ -355,7 +355,6 @@ __device__ __forceinline__ bool softmax_rows(Smem<HD>& sm, int w, uint32_t s_add
 // arrives as zeros.  Issuing is the bound (about 45 ns per copy of a warp, whatever other warps do): one warp per stream
 // took 3 us for a tile, so four warps share both.  (Copied by 128 threads with cp.async, 16 bytes at a time, a tile took
 // 2 to 4 us beside the softmax warps, whose issue slots those copies also take.)
-enum Mode { kWindow, kPrefixPair, kPrefixSplit };      // kPrefixSplit: AttendParams::key_split
 template <typename T, int HD, int kMode, bool E4>
 __global__ void __launch_bounds__(kThreads, 1)
 attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -363,10 +362,11 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     constexpr bool kPrefix = kMode != kWindow, key_split = kMode == kPrefixSplit;
     using MT = typename std::conditional<E4, __half, T>::type;       // e4m3 rows are multiplied as fp16
     using R = Cfg<E4>;
-    constexpr int kTileBytes = Smem<HD>::kTile;
+    using SM = Smem<HD, kMode, E4>;
+    constexpr int kTileBytes = SM::kTile, kStages = SM::kStages;
     constexpr int QC = HD / 8;                                       // 16-byte chunks of a query row
     extern __shared__ unsigned char smem_raw[];
-    Smem<HD>& sm = *reinterpret_cast<Smem<HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    SM& sm = *reinterpret_cast<SM*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     AbortBox* const wc = &sm.box;
     const int G = p.H / p.Hkv;
@@ -503,21 +503,25 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
         }
     };
-    // Slots -> rows to gather; `mark`: notes which rows of the tile (the CTA's t-th) there are none for.  bad[t & 3] is
-    // read until the tile's P is there, which the MMA thread waits for before it issues anything of two tiles later
-    // and so before the release that lets the tile after next but one in.
+    // Slots -> rows to gather; `mark`: notes which rows of the tile (the CTA's t-th) there are none for, a word per eight
+    // lanes.  bad[t & 7] is read until the tile's P is there; the MMA thread waits for that before it issues anything of
+    // four tiles later, and so before the release that lets a tile into this place again.
     auto to_rows = [&](const Slots& sl, int j, int t, int r0, const int (&x)[4], int (&row)[4], bool mark) {
-        bool bad = false;
-        uint32_t bytes = 0;
+        uint32_t none = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const bool in = x[i] >= 0 && x[i] < sl.n_slots;
-            bad |= !in && r0 + i < tile_keys(sl.w0, j);
-            bytes |= in ? 0u : 1u << (8 * i);
+            none |= in ? 0u : 1u << i;
             row[i] = in ? x[i] : sl.n_slots;
         }
-        if (mark && (E4 || lane < 8)) {
-            *reinterpret_cast<uint32_t*>(&sm.bad[t & 3][r0]) = bytes;
+        if (mark) {
+            const int keys = tile_keys(sl.w0, j) - r0;                    // those of the four that are keys at all
+            const bool bad = none & (keys >= 4 ? 15u : keys <= 0 ? 0u : (1u << keys) - 1u);
+            none <<= (r0 & 31);
+            none |= __shfl_xor_sync(0xffffffffu, none, 1);
+            none |= __shfl_xor_sync(0xffffffffu, none, 2);
+            none |= __shfl_xor_sync(0xffffffffu, none, 4);
+            if ((lane & 7) == 0 && (E4 || lane == 0)) sm.bad[t & 7][r0 >> 5] = none;
             if (bad) {
                 sm.any_bad = 1;
                 if (p.err_flag) atomicOr(p.err_flag, ATTN_B200_FLAG_BAD_SLOT);
@@ -680,9 +684,9 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 // W: the warpgroup, a compile-time 0 or 1, so that all of this stays in registers
                 auto start_tile = [&](auto W, int t, int wide) -> bool {                  // Q.K of tile t (of the CTA)
                     constexpr int w = decltype(W)::value;
-                    if (!mbar_wait(&sm.k_full[t & 1], (t >> 1) & 1, wc)) return false;
+                    if (!mbar_wait(&sm.k_full[t % kStages], (t / kStages) & 1, wc)) return false;
                     tc_fence_after();
-                    const uint64_t a = qd + (w ? (key_split ? 0 : kTile16) : 0), b2 = kd + (t & 1) * kTile16;
+                    const uint64_t a = qd + (w ? (key_split ? 0 : kTile16) : 0), b2 = kd + (t % kStages) * kTile16;
                     const uint32_t idesc = idesc0 | ((uint32_t)(wide >> 3) << 17);
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk) {
@@ -697,11 +701,11 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     int& done = w ? done1 : done0;
                     const uint32_t ph = done & 1;
                     ++done;
-                    const uint64_t v = vd + (t & 1) * kTile16;
+                    const uint64_t v = vd + (t % kStages) * kTile16;
                     const uint32_t d = tmem + 256 + w * 128, a = tmem + w * 128;
                     if (first && (w ? uses1 : uses0) > 0 && !mbar_wait(&sm.o_free[w], ((w ? uses1 : uses0) - 1) & 1, wc)) return false;
                     if (!mbar_wait(&sm.p_half[w], ph, wc)) return false;
-                    if (!mbar_wait(&sm.v_full[t & 1], (t >> 1) & 1, wc)) return false;
+                    if (!mbar_wait(&sm.v_full[t % kStages], (t / kStages) & 1, wc)) return false;
                     tc_fence_after();
                     if (wide == BN) {
 #pragma unroll
@@ -739,17 +743,17 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         }
                         for (int j = 0; ok && j < tiles; j += 2) {
                             if (!(ok = finish_tile(W0, j, wide(j), j == 0))) break;
-                            umma_commit(&sm.v_empty[0]);
+                            umma_commit(&sm.v_empty[j % kStages]);
                             if (j + 2 < tiles) {
                                 if (!(ok = start_tile(W0, j + 2, BN))) break;
-                                umma_commit(&sm.k_empty[0]);
+                                umma_commit(&sm.k_empty[(j + 2) % kStages]);
                             }
                             if (j + 1 == tiles) break;
                             if (!(ok = finish_tile(W1, j + 1, BN, j == 0))) break;
-                            umma_commit(&sm.v_empty[1]);
+                            umma_commit(&sm.v_empty[(j + 1) % kStages]);
                             if (j + 3 < tiles) {
                                 if (!(ok = start_tile(W1, j + 3, BN))) break;
-                                umma_commit(&sm.k_empty[1]);
+                                umma_commit(&sm.k_empty[(j + 3) % kStages]);
                             }
                         }
                     } else {
@@ -761,7 +765,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                             ok = start_tile(W1, g, wide0);
                             if (je1 == 1) umma_commit(&sm.q_empty[1]);
                         }
-                        umma_commit(&sm.k_empty[g & 1]);
+                        umma_commit(&sm.k_empty[g % kStages]);
                         for (int j = 0; ok && j < tiles; ++j) {
                             const int t = g + j;
                             if (j >= jb0 && j < je0 && !(ok = finish_tile(W0, t, wide(j), j == jb0))) break;
@@ -770,12 +774,12 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                                 if (j + 2 == je0) umma_commit(&sm.q_empty[0]);
                             }
                             if (j >= jb1 && j < je1 && !(ok = finish_tile(W1, t, wide(j), j == jb1))) break;
-                            umma_commit(&sm.v_empty[t & 1]);
+                            umma_commit(&sm.v_empty[t % kStages]);
                             if (j + 1 >= jb1 && j + 1 < je1) {
                                 if (!(ok = start_tile(W1, t + 1, BN))) break;
                                 if (j + 2 == je1) umma_commit(&sm.q_empty[1]);
                             }
-                            if (j + 1 < tiles) umma_commit(&sm.k_empty[(t + 1) & 1]);
+                            if (j + 1 < tiles) umma_commit(&sm.k_empty[(t + 1) % kStages]);
                         }
                     }
                     if (!ok) break;
@@ -859,41 +863,51 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             // store instruction touches 32 rows.
             const int lr = lane, row_w = it.row0[w] + (warp & 3) * 32;       // this warp's first row
             if (kPrefix) {
+                // Partial rows lie by KV head, [n_parts, Hkv, B * G, HD], so that a warp's 32 rows are one box of a TMA
+                // store per 32 columns.  Staged where this warpgroup's last K tile (its query tile) was.
                 const float vs = E4 ? p.v_scale[it.hk] : 1.f;
-                const int64_t set = (int64_t)p.B * p.H, part = it.part + (key_split ? w : 0);
-                float2* const ml = reinterpret_cast<float2*>(p.parts + (int64_t)attend_prefix_parts(p) * set * HD);
-                const uint32_t buf = smem_u32(sm.q[w]) + (warp & 3) * (kTileBytes / 4);
-                constexpr int kCols = kTileBytes / BM / 4;                  // floats per row and pass
+                const int64_t rows_all = (int64_t)p.B * p.H, part = it.part + (key_split ? w : 0);
+                const int64_t row0 = part * rows_all + (int64_t)it.hk * it.n_rows;        // first row of the KV head's block
+                const int last = it.tiles - 1 - ((it.tiles - 1 + w) & 1);                 // key_split: this warpgroup's last tile, or -1
+                unsigned char* const stage = (key_split ? sm.k[(last + kStages) % kStages] : sm.q[key_split ? 0 : w]) + (warp & 3) * (kTileBytes / 4);
+                constexpr int kBoxes = kTileBytes / 4 / 4096;                             // boxes that fit the warp's share
+                const bool box = row_w + 32 <= it.n_rows;
 #pragma unroll
-                for (int c = 0; c < HD; c += kCols) {
-                    const uint32_t mine = buf + lr * (kCols * 4);
+                for (int c = 0; c < HD; c += 32) {
+                    const uint32_t buf = smem_u32(stage) + (c / 32 % kBoxes) * 4096;
+                    if (c >= 32 * kBoxes) {
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kBoxes - 1) : "memory");
+                        __syncwarp();
+                    }
+                    float ov[32];
                     if (count > 0) {
-                        float ov[kCols];
-#pragma unroll
-                        for (int e = 0; e < kCols; e += 32) tmem_ld32(o_addr + c + e, ov + e);
-#pragma unroll
-                        for (int e = 0; e < kCols / 4; ++e)
-                            st_shared16(mine + ((e ^ (lr & (kCols / 4 - 1))) << 4), __float_as_uint(ov[4 * e] * vs), __float_as_uint(ov[4 * e + 1] * vs),
-                                        __float_as_uint(ov[4 * e + 2] * vs), __float_as_uint(ov[4 * e + 3] * vs));
+                        tmem_ld32(o_addr + c, ov);
                     } else {
-                        for (int e = 0; e < kCols / 4; ++e) st_shared16(mine + (e << 4), 0, 0, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) ov[e] = 0.f;
                     }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        st_shared16(buf + lr * 128 + ((e ^ (lr & 7)) << 4), __float_as_uint(ov[4 * e] * vs), __float_as_uint(ov[4 * e + 1] * vs),
+                                    __float_as_uint(ov[4 * e + 2] * vs), __float_as_uint(ov[4 * e + 3] * vs));
+                    if (box) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    constexpr int kLanes = kCols / 4, kRows = 32 / kLanes;   // lanes per row, rows per store
-                    Rows rows = rows_from(it, w, row_w + lane / kLanes);
-                    float* const dst = p.parts + part * set * HD + c + lane % kLanes * 4;
-#pragma unroll 8
-                    for (int i = 0; i < 32; i += kRows) {
-                        const int rr = i + lane / kLanes, cc = lane % kLanes;
-                        const uint4 x = ld_shared16(buf + rr * (kCols * 4) + ((cc ^ (rr & (kLanes - 1))) << 4));
-                        const int64_t at = rows.at();
-                        if (at >= 0) *reinterpret_cast<uint4*>(dst + at) = x;
-                        rows.next(kRows);
+                    if (box) {
+                        if (lane == 0) {
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+                                         ::"l"(reinterpret_cast<uint64_t>(&map_o)), "r"(c), "r"((int)(row0 + row_w)), "r"(buf) : "memory");
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int i = lane / 8; i < 32 && row_w + i < it.n_rows; i += 4)
+                            *reinterpret_cast<uint4*>(p.parts + (row0 + row_w + i) * HD + c + lane % 8 * 4) =
+                                ld_shared16(buf + i * 128 + ((lane % 8 ^ (i & 7)) << 4));
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
-                const int64_t at = rows_from(it, w, row).at();
-                if (at >= 0) ml[part * set + at / HD] = make_float2(count > 0 ? m : -INFINITY, l);
+                float2* const ml = reinterpret_cast<float2*>(p.parts + (int64_t)attend_prefix_parts(p) * rows_all * HD);
+                if (row < it.n_rows) ml[row0 + row] = make_float2(count > 0 ? m : -INFINITY, l);
             } else if (count > 0) {
                 float ov[HD];
 #pragma unroll
@@ -944,7 +958,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
             done_with(n);
         }
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // shared memory stays until the stores have read it
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");           // the stores are done before the CTA is
     }
     tc_fence_before();
     __syncthreads();
@@ -998,7 +1012,6 @@ int launch_dependent(void (*kernel)(K...), dim3 grid, int threads, int smem, cud
     return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-static_assert(sizeof(Smem<128>) + 1024 <= 227 * 1024, "shared memory");
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -1018,7 +1031,10 @@ int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(cols * elem_bytes)};
     const cuuint32_t box[2] = {(cuuint32_t)width, (cuuint32_t)height}, step[2] = {1, 1};
     // the copies move bits: every 16-bit type is taken as fp16
-    const CUresult r = fn(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
+    const CUtensorMapDataType type = elem_bytes == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims,
                           strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
@@ -1027,7 +1043,8 @@ int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int
 template <typename T, int HD, int kMode, bool E4>
 int launch(const AttendParams& p, dim3 grid, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
-    const int smem = (int)sizeof(Smem<HD>) + 1024;
+    constexpr int smem = (int)sizeof(Smem<HD, kMode, E4>) + 1024;
+    static_assert(smem <= 227 * 1024, "shared memory");
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
@@ -1048,7 +1065,10 @@ int launch(const AttendParams& p, dim3 grid, cudaStream_t st) {
             (rc = make_map(&mo, p.out, p.n_q_tokens, (int64_t)p.H * HD, 2, 64, 32, true)))
             return rc;
     } else {
-        mq = mo = mk;          // not used
+        mq = mk;               // not used
+        const int64_t rows = (int64_t)attend_prefix_parts(p) * p.B * p.H;
+        if (rows > 0x7fffffffLL) return ATTN_B200_ETOOLARGE;
+        if ((rc = make_map(&mo, p.parts, rows, HD, 4, 32, 32, true))) return rc;
     }
     return launch_dependent(attend_tc_kernel<T, HD, kMode, E4>, grid, kThreads, smem, st, mq, mk, mv, mo, p);
 }

@@ -21,7 +21,7 @@ struct AttendParams {
     int blocks, units;               // query blocks of the longest chunk, head units: set by the launcher
     int64_t n_items;
     // prefix
-    float* parts;                    // o [n_parts, B, H, D], then (m, l) [n_parts, B, H]
+    float* parts;                    // o [n_parts, Hkv, B * G, D], then (m, l) [n_parts, Hkv, B * G]
     int n_prefix, splits, key_split;
     const float *k_scale, *v_scale;
 };

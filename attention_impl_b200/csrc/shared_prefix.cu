@@ -87,9 +87,9 @@ extern "C" int attn_b200_shared_prefix_decode(const void* q, const void* k_new, 
         p.parts = a.parts;
         p.n_parts = parts;
         p.early = 1;
-        return span_decode_launch(p, n_tokens / B + 1, q_dtype, kv_dtype, st);
+        return span_decode_launch(p, n_tokens / B + 1, B > 1, q_dtype, kv_dtype, st);
     }
     p.prefix = prefix_slots;
     p.n_prefix = (int)n_prefix;
-    return span_decode_launch(p, n_prefix + n_tokens / B + 1, q_dtype, kv_dtype, st);
+    return span_decode_launch(p, n_prefix + n_tokens / B + 1, B > 1 && n_tokens > B * n_prefix, q_dtype, kv_dtype, st);
 }

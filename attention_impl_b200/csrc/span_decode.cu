@@ -151,7 +151,8 @@ __device__ __forceinline__ void fold(const SpanParams& p, FoldWeights& fw, int b
     const int G = p.H / p.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float* const weight = &fw.worker[0][0];                  // [hpc * heads][workers]
     const int64_t set = (int64_t)p.B * p.H;
-    const float2* const pml = reinterpret_cast<const float2*>(p.parts + p.n_parts * set * D) + (int64_t)b * p.H;
+    const float2* const pml = reinterpret_cast<const float2*>(p.parts + p.n_parts * set * D);
+    auto part_row = [&](int h) { return ((int64_t)(h / G) * p.B + b) * G + h % G; };      // of the first partial set
     auto head_of = [&](int gh) -> int {                      // query head of this CTA's gh-th, or -1
         const int slot = gh / heads, vh = vh0 + slot, hk = vh / p.n_sets, g = (vh - hk * p.n_sets) * 8 + gh - slot * heads;
         return hk < p.Hkv && g < G ? hk * G + g : -1;
@@ -169,7 +170,8 @@ __device__ __forceinline__ void fold(const SpanParams& p, FoldWeights& fw, int b
             if (w < workers) v[i] = ld_cluster2(in_cta(ml + (warp_of * heads + gh - slot * heads) * 8, w >> wph_log2));
             M = fmaxf(M, v[i].x);
         }
-        for (int k = lane; k < p.n_parts; k += 32) M = fmaxf(M, pml[k * set + h].x);
+        const float2* const pm = pml + part_row(h);
+        for (int k = lane; k < p.n_parts; k += 32) M = fmaxf(M, pm[k * set].x);
         M = group_max<32>(M);
         if (!(M > -INFINITY)) M = 0.f;                       // nothing but -inf: 0 / 0 below, as the formula has it
         float e[2], den = 0.f;
@@ -179,7 +181,7 @@ __device__ __forceinline__ void fold(const SpanParams& p, FoldWeights& fw, int b
             den += e[i] * v[i].y;
         }
         for (int k = lane; k < p.n_parts; k += 32) {
-            const float2 x = pml[k * set + h];
+            const float2 x = pm[k * set];
             den += fast_exp2(x.x - M) * x.y;
         }
         const float fresh = fast_exp2(sn - M);
@@ -207,9 +209,10 @@ __device__ __forceinline__ void fold(const SpanParams& p, FoldWeights& fw, int b
 #pragma unroll 4
             for (int w = sub; w < workers; w += share)
                 add4(o, weight[gh * workers + w], ld_cluster4(in_cta(part0 + (w & ((1 << wph_log2) - 1)) * part_stride, w >> wph_log2)));
-            const float4* po = reinterpret_cast<const float4*>(p.parts + ((int64_t)b * p.H + h) * D + d);
+            const int64_t row = part_row(h);
+            const float4* po = reinterpret_cast<const float4*>(p.parts + row * D + d);
 #pragma unroll 12
-            for (int k = sub; k < p.n_parts; k += share) add4(o, fast_exp2(pml[k * set + h].x - fw.top[gh]) * fw.inv[gh], po[k * set * (D / 4)]);
+            for (int k = sub; k < p.n_parts; k += share) add4(o, fast_exp2(pml[k * set + row].x - fw.top[gh]) * fw.inv[gh], po[k * set * (D / 4)]);
         }
         for (int m = 1; m < share; m <<= 1) {
             o.x += __shfl_xor_sync(0xffffffffu, o.x, m);
@@ -232,7 +235,7 @@ template <int D, bool E4> struct Ring {
     static constexpr int kRow = E4 ? D : 2 * D;                  // bytes of a head's K (or V) row
     static constexpr int J = kRow / 64;                          // 16-byte chunks of a row per lane
     static constexpr int kStageBytes = kTile * 2 * kRow;
-    static constexpr int kStages = kStageBytes > 8192 ? 2 : 3;
+    static constexpr int kStages = kStageBytes > 4096 ? 2 : 3;   // D = 128, 16 bits: 3 CTAs of 2 per SM beat 2 of 3 (187 against 207 us, batch 64)
     static constexpr int kWarpBytes = kStages * kStageBytes;
     static constexpr int kBytes = kWarps * kWarpBytes;
     static constexpr int kCtasPerSm = 227 * 1024 / (kBytes + 4096) < 4 ? 227 * 1024 / (kBytes + 4096) : 4;
@@ -593,26 +596,29 @@ int launch(K kernel, const SpanParams& p, int64_t units, int smem, cudaStream_t 
 }
 
 template <typename T, int D, bool E4>
-int launch_mma(SpanParams p, int64_t span, cudaStream_t st) {
+int launch_mma(SpanParams p, int64_t span, bool ragged, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
     const int G = p.H / p.Hkv;
     p.n_sets = (G + 7) / 8;
     const int vheads = p.Hkv * p.n_sets;
-    // Heads per CTA and CTAs per sequence: one wave of CTAs, as full as a power of two makes it (a second wave
-    // costs a CTA's whole start and end, ~6 us; a cluster of 16 about 10 more).  Few heads per CTA (several warps to a head)
-    // start and end quickest: batch 8, 32 KV heads, 512 tokens 16.2 us with one head per CTA, 18.3 with four and
-    // clusters of four.  Four adjacent heads read 4 times the contiguous bytes per token, which counts once DRAM is
-    // the bound: batch 64, 8 KV heads, 4100 tokens 207 us with four heads and clusters of two, 258 with two, 356 with one.
+    // Heads per CTA and CTAs per sequence: one wave of CTAs, as full as whole splits make it (a second wave costs a
+    // CTA's whole start and end, ~6 us; a cluster of 16 about 10 more).  Few heads per CTA (several warps to a head)
+    // start and end quickest: batch 8, 32 KV heads, 512 tokens 16.9 us with one head per CTA, 18 to 20 with four.  Four
+    // adjacent heads read 4 times the contiguous bytes per token, which counts once DRAM is the bound: batch 64, 8 KV
+    // heads, 4100 tokens 187 us with four heads and clusters of three, 258 with two, 349 with one.  Sequences of very
+    // different lengths want many small CTAs: 64 with 16 to 1024 tokens, 36 us with one head per CTA, 52 with four.
     const int64_t slots = 148 * Ring<D, E4>::kCtasPerSm, tiles = (span + kTile - 1) / kTile;
     const int64_t bytes = (int64_t)p.B * span * 2 * p.Hkv * Ring<D, E4>::kRow;
     auto units_of = [&](int hl) { return (int64_t)p.B * ((vheads + (1 << hl) - 1) >> hl); };
     auto splits_of = [&](int hl) {
-        int s = 1;
-        while (s < 16 && units_of(hl) * s * 2 <= slots && tiles > (int64_t)s * (kWarps >> hl)) s *= 2;
-        return s;
+        const int64_t fit = slots / units_of(hl), most = (tiles + (kWarps >> hl) - 1) / (kWarps >> hl);
+        const int64_t s = fit < most ? fit : most;
+        return s >= 16 ? 16 : s > 8 ? 8 : s < 1 ? 1 : (int)s;
     };
     int hl = 0;
-    while (hl < 2 && (2 << hl) <= vheads && (units_of(hl) > slots || (bytes > (100 << 20) && splits_of(hl + 1) <= 4))) ++hl;
+    while (hl < 2 && (2 << hl) <= vheads &&
+           (units_of(hl) > (ragged ? 2 * slots : slots) || (!ragged && bytes > (100 << 20) && splits_of(hl + 1) <= 4)))
+        ++hl;
     const int64_t units = units_of(hl);
     const int s = splits_of(hl);
     p.hpc_log2 = hl;
@@ -640,13 +646,13 @@ int launch_generic(const SpanParams& p, int64_t span, cudaStream_t st) {
 }
 
 template <typename T>
-int dispatch16(const SpanParams& p, int64_t span, bool e4, cudaStream_t st) {
+int dispatch16(const SpanParams& p, int64_t span, bool ragged, bool e4, cudaStream_t st) {
     const bool aligned = (((uintptr_t)p.q | (uintptr_t)p.k_new | (uintptr_t)p.k_cache | (uintptr_t)p.v_cache) & 15) == 0;
     if (aligned) {
         switch (p.D) {
-            case 64: return e4 ? launch_mma<T, 64, true>(p, span, st) : launch_mma<T, 64, false>(p, span, st);
-            case 128: return e4 ? launch_mma<T, 128, true>(p, span, st) : launch_mma<T, 128, false>(p, span, st);
-            case 256: return e4 ? launch_mma<T, 256, true>(p, span, st) : launch_mma<T, 256, false>(p, span, st);
+            case 64: return e4 ? launch_mma<T, 64, true>(p, span, ragged, st) : launch_mma<T, 64, false>(p, span, ragged, st);
+            case 128: return e4 ? launch_mma<T, 128, true>(p, span, ragged, st) : launch_mma<T, 128, false>(p, span, ragged, st);
+            case 256: return e4 ? launch_mma<T, 256, true>(p, span, ragged, st) : launch_mma<T, 256, false>(p, span, ragged, st);
             default: break;
         }
     }
@@ -656,11 +662,11 @@ int dispatch16(const SpanParams& p, int64_t span, bool e4, cudaStream_t st) {
 
 }  // namespace
 
-int span_decode_launch(SpanParams p, int64_t span, int q_dtype, int kv_dtype, cudaStream_t st) {
+int span_decode_launch(SpanParams p, int64_t span, bool ragged, int q_dtype, int kv_dtype, cudaStream_t st) {
     const bool e4 = kv_dtype == ATTN_B200_E4M3;
     switch (q_dtype) {
-        case ATTN_B200_F16: return dispatch16<__half>(p, span, e4, st);
-        case ATTN_B200_BF16: return dispatch16<__nv_bfloat16>(p, span, e4, st);
+        case ATTN_B200_F16: return dispatch16<__half>(p, span, ragged, e4, st);
+        case ATTN_B200_BF16: return dispatch16<__nv_bfloat16>(p, span, ragged, e4, st);
         case ATTN_B200_F32: return p.n_parts ? ATTN_B200_ESHAPE : launch_generic<float, float>(p, span, st);
         default: return ATTN_B200_EDTYPE;
     }
@@ -695,6 +701,8 @@ extern "C" int attn_b200_paged_window_decode(const void* q, const void* k_new, c
     p.k_scale = kv_dtype == ATTN_B200_E4M3 ? k_scale : nullptr;
     p.v_scale = kv_dtype == ATTN_B200_E4M3 ? v_scale : nullptr;
     p.err_flag = err_flag;
-    const int64_t seen = (int64_t)window - 1 + n_sinks, longest = block_size > 1 ? (int64_t)max_blocks * block_size : n_tokens;
-    return span_decode_launch(p, seen < longest ? seen : longest, q_dtype, kv_dtype, (cudaStream_t)stream);
+    // most sequences are taken to fill the span unless the table shows that they cannot
+    const int64_t seen = (int64_t)window - 1 + n_sinks, average = block_size > 1 ? (int64_t)max_blocks * block_size : n_tokens / B;
+    const bool ragged = B > 1 && average < 2 * seen;
+    return span_decode_launch(p, average < seen ? average + 1 : seen, ragged, q_dtype, kv_dtype, (cudaStream_t)stream);
 }

@@ -13,7 +13,7 @@ struct SpanParams {
     const int32_t* prefix;              // slots of rows that every sequence sees before its own
     int n_prefix;
     void* out;
-    const float* parts;                 // to fold in, or null: o [n_parts, B, H, D], then (m (log2 domain), l) [n_parts, B, H]
+    const float* parts;                 // to fold in, or null: o [n_parts, Hkv, B * G, D], then (m (log2), l) [n_parts, Hkv, B * G]
     int n_parts;
     int B, H, Hkv, D;
     int64_t n_tokens, n_slots;          // entries of a per-token table; pool rows
@@ -27,7 +27,8 @@ struct SpanParams {
     int hpc_log2, n_sets, splits;
 };
 
-// `span_hint`: an upper estimate of the cached tokens that a sequence attends to (only for the split).
-int span_decode_launch(SpanParams p, int64_t span_hint, int q_dtype, int kv_dtype, cudaStream_t st);
+// `span`: an estimate of the cached tokens that a sequence attends to; `ragged`: an average of very different numbers,
+// not a bound that most sequences reach (both only for the split).
+int span_decode_launch(SpanParams p, int64_t span, bool ragged, int q_dtype, int kv_dtype, cudaStream_t st);
 
 }  // namespace attn
