@@ -108,19 +108,27 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
     return x;
 }
 
-// Item `id` of a window launch (false: it has no query rows)
-__device__ __forceinline__ bool window_item(const AttendParams& p, int64_t id, Item& it) {
-    const int64_t bb = id / p.units;
-    const int unit = (int)(id - bb * p.units), b = (int)(bb / p.blocks), blk = (int)(bb - (int64_t)b * p.blocks), G = p.H / p.Hkv;
+// Blocks of query rows of sequence b (window); a sequence whose offsets make no sense has none
+__device__ __forceinline__ int window_blocks(const AttendParams& p, int b) {
+    if (b >= p.B) return 0;
     const int64_t q_beg = b ? p.q_offsets[b - 1] : 0, q_end = p.q_offsets[b];
     const int64_t kv_beg = b ? p.kv_offsets[b - 1] : 0, kv_end = p.kv_offsets[b];
     if (q_beg < 0 || q_end < q_beg || q_end > p.n_q_tokens || kv_beg < 0 || kv_end > p.n_kv_tokens || kv_end - kv_beg < q_end - q_beg) {
         if (p.err_flag) atomicOr(p.err_flag, ATTN_B200_FLAG_BAD_OFFSETS);
-        return false;
+        return 0;
     }
+    const int rows = p.head_pairs ? BM : 2 * BM;
+    const int64_t n = (q_end - q_beg + rows - 1) / rows;
+    return (int)(n < p.blocks ? n : p.blocks);
+}
+
+// Block `blk` of sequence b for head unit `unit` (the sequence's offsets are good and it has that block)
+__device__ __forceinline__ void window_item(const AttendParams& p, int b, int blk, int unit, Item& it) {
+    const int G = p.H / p.Hkv;
+    const int64_t q_beg = b ? p.q_offsets[b - 1] : 0, q_end = p.q_offsets[b];
+    const int64_t kv_beg = b ? p.kv_offsets[b - 1] : 0, kv_end = p.kv_offsets[b];
     const int q_len = (int)(q_end - q_beg), kv_len = (int)(kv_end - kv_beg), shift = kv_len - q_len;
     const int rows = p.head_pairs ? BM : 2 * BM, q0 = blk * rows;
-    if (q0 >= q_len) return false;
     if (p.head_pairs) {
         it.hk = unit / (G / 2);
         it.head[0] = unit * 2;
@@ -150,7 +158,6 @@ __device__ __forceinline__ bool window_item(const AttendParams& p, int64_t id, I
     it.n_rows = q_len;
     it.shift = shift;
     it.q_beg = q_beg;
-    return true;
 }
 
 // The one item of a prefix CTA: its share of the key tiles (the list's first tile is the short one) for a pair
@@ -651,23 +658,51 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::kOther));
         if (warp == 8) {
             // -------------------------------------------------------------- item list
-            if (lane == 0) {
-                int64_t id = blockIdx.x;
-                for (int n = 0;; ++n) {
-                    if (n >= kItems && !mbar_wait(&sm.item_empty[n % kItems], (n / kItems - 1) & 1, wc)) break;
+            // The items of a window launch are the existing blocks of all sequences times the head units, the unit changing
+            // fastest (its CTAs share K and V); this CTA takes every gridDim.x-th.  The warp looks at 32 sequences at a
+            // time, once each, so empty and short chunks cost next to nothing.
+            int base = 0, mine = 0, upto = 0, before = 0;       // sequences base .. base + 31: blocks of lane's, scan of them, blocks ahead of base
+            auto look = [&] {
+                mine = window_blocks(p, base + lane);
+                upto = mine;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int x = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (lane >= d) upto += x;
+                }
+            };
+            if (!kPrefix) look();
+            for (int n = 0;; ++n) {
+                bool end = kPrefix && n > 0;
+                int b = 0, blk = 0, unit = 0;
+                if (!kPrefix) {
+                    const int64_t id = blockIdx.x + (int64_t)n * gridDim.x, block = id / p.units;
+                    unit = (int)(id - block * p.units);
+                    while (!end && block >= before + (int64_t)__shfl_sync(0xffffffffu, upto, 31)) {
+                        before += __shfl_sync(0xffffffffu, upto, 31);
+                        base += 32;
+                        if (base >= p.B) end = true;
+                        else look();
+                    }
+                    if (!end) {
+                        const int in = (int)(block - before);
+                        const int src = __ffs(__ballot_sync(0xffffffffu, upto > in)) - 1;
+                        b = base + src;
+                        blk = in - __shfl_sync(0xffffffffu, upto - mine, src);
+                    }
+                }
+                bool ok = n < kItems || mbar_wait(&sm.item_empty[n % kItems], (n / kItems - 1) & 1, wc);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                if (lane == 0) {
                     Item& it = sm.item[n % kItems];
                     it.tiles = 0;
-                    if (kPrefix) {
-                        if (n == 0) prefix_item(p, it);
-                    } else {
-                        bool found = false;
-                        for (; id < p.n_items && !found; id += gridDim.x) found = window_item(p, id, it);
-                        if (!found) it.tiles = 0;
+                    if (!end) {
+                        if constexpr (kPrefix) prefix_item(p, it);
+                        else window_item(p, b, blk, unit, it);
                     }
-                    const bool end = it.tiles == 0;
                     mbar_arrive(&sm.item_full[n % kItems]);
-                    if (end) break;
                 }
+                if (end) break;
             }
         } else if (warp == 9) {
             // -------------------------------------------------------------- MMA issuer
@@ -1093,8 +1128,9 @@ int attend_window_launch(AttendParams p, int max_q_len, int D, int dtype, cudaSt
     if (blocks == 0 || p.B == 0) return 0;
     p.blocks = blocks;
     p.units = units;
-    p.n_items = (int64_t)blocks * units * p.B;
-    const dim3 grid((unsigned)(p.n_items < 148 ? p.n_items : 148));       // one CTA per SM
+    // one CTA per SM, no more than there can be items
+    const int64_t most = (p.n_q_tokens / rows + p.B) * units, sms = current_sm_count();
+    const dim3 grid((unsigned)(most < sms ? most : sms));
     const bool bf = dtype == ATTN_B200_BF16;
     if (D == 64) return bf ? launch<__nv_bfloat16, 64, kWindow, false>(p, grid, st) : launch<__half, 64, kWindow, false>(p, grid, st);
     return bf ? launch<__nv_bfloat16, 128, kWindow, false>(p, grid, st) : launch<__half, 128, kWindow, false>(p, grid, st);
@@ -1107,10 +1143,11 @@ void attend_prefix_plan(AttendParams& p) {
     const int tiles = (p.n_prefix + BN - 1) / BN;
     // one CTA per SM: the number of splits with the fewest tile steps in the longest chain; a wave costs
     // about three steps besides (set-up, first rows, partial rows)
+    const int sms = current_sm_count();
     int64_t best = -1;
     p.splits = 1;
-    for (int s = 1; s <= 148 && s <= tiles; ++s) {
-        const int64_t cost = (items * s + 147) / 148 * ((tiles + s - 1) / s + 3);
+    for (int s = 1; s <= sms && s <= tiles; ++s) {
+        const int64_t cost = (items * s + sms - 1) / sms * ((tiles + s - 1) / s + 3);
         if (best < 0 || cost < best) {
             best = cost;
             p.splits = s;

@@ -19,7 +19,6 @@ struct AttendParams {
     int64_t n_q_tokens, n_kv_tokens;
     int window, sinks, head_pairs;
     int blocks, units;               // query blocks of the longest chunk, head units: set by the launcher
-    int64_t n_items;
     // prefix
     float* parts;                    // o [n_parts, Hkv, B * G, D], then (m, l) [n_parts, Hkv, B * G]
     int n_prefix, splits, key_split;

@@ -90,4 +90,20 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return y;
 }
 
+// ---------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------
+// SMs of the current device (looked up once per device)
+inline int current_sm_count() {
+    static int known[64];                // written with the same value by whoever comes first
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    int n = __atomic_load_n(&known[dev], __ATOMIC_RELAXED);
+    if (n == 0) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+        __atomic_store_n(&known[dev], n, __ATOMIC_RELAXED);
+    }
+    return n;
+}
+
 }  // namespace attn

@@ -135,7 +135,6 @@ __device__ __forceinline__ bool token_ok(const NormRopeParams& p, int64_t token,
 // with the next round's loads ahead of the arithmetic and five CTAs per SM = 5.6 TB/s, 0.86 of the
 // measured copy rate; with the append (940 MB) 222 -> 158 us = 5.9 TB/s.
 constexpr int kThreads = 128, kUnroll = 2, kCtasPerSm = 5, kRounds = 4;
-constexpr int64_t kFillThreads = 148 * 5 * 128;
 
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     float2 d;
@@ -369,9 +368,10 @@ template <typename T> int launch(const NormRopeParams& p0, cudaStream_t st) {
         // kRounds rounds over the q heads, which pays for its coefficients (16384 tokens, 32 + 32 heads of
         // 128, fp16: 102 us with four rounds, 109 with two, 110 with eight) - unless there are too few
         // tokens to fill the machine that way (8 tokens: 3.7 us with one round, 7 with four).
+        const int64_t fill = (int64_t)current_sm_count() * kCtasPerSm * kThreads;
         int tl = 0;
         while ((1 << tl) < kThreads && ((1 << tl) < lph || (1 << tl) * kRounds * kUnroll < p.hq * lph)) ++tl;
-        while ((1 << tl) < kThreads && (1 << tl) * kUnroll < p.hq * lph && (p.n_tokens << tl) < kFillThreads) ++tl;
+        while ((1 << tl) < kThreads && (1 << tl) * kUnroll < p.hq * lph && (p.n_tokens << tl) < fill) ++tl;
         p.tpt_log2 = tl;
         const int64_t per_cta = kThreads >> tl, ctas = (p.n_tokens + per_cta - 1) / per_cta;
         if (ctas > 0x7fffffff) return ATTN_B200_ETOOLARGE;

@@ -607,7 +607,7 @@ int launch_mma(SpanParams p, int64_t span, bool ragged, cudaStream_t st) {
     // adjacent heads read 4 times the contiguous bytes per token, which counts once DRAM is the bound: batch 64, 8 KV
     // heads, 4100 tokens 187 us with four heads and clusters of three, 258 with two, 349 with one.  Sequences of very
     // different lengths want many small CTAs: 64 with 16 to 1024 tokens, 36 us with one head per CTA, 52 with four.
-    const int64_t slots = 148 * Ring<D, E4>::kCtasPerSm, tiles = (span + kTile - 1) / kTile;
+    const int64_t slots = (int64_t)current_sm_count() * Ring<D, E4>::kCtasPerSm, tiles = (span + kTile - 1) / kTile;
     const int64_t bytes = (int64_t)p.B * span * 2 * p.Hkv * Ring<D, E4>::kRow;
     auto units_of = [&](int hl) { return (int64_t)p.B * ((vheads + (1 << hl) - 1) >> hl); };
     auto splits_of = [&](int hl) {
@@ -631,7 +631,7 @@ int launch_generic_d(SpanParams p, int64_t span, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
     const int64_t units = (int64_t)p.B * p.H;
     int s = 1;
-    while (s < 8 && units * s < 148 * 4 && span > (int64_t)s * kWarps * 8) s *= 2;
+    while (s < 8 && units * s < current_sm_count() * 4 && span > (int64_t)s * kWarps * 8) s *= 2;
     p.splits = s;
     p.n_sets = 1;
     return launch(span_decode_generic_kernel<T, KV, DPL>, p, units, kWarps * 32 * DPL * 4, st, ready);

@@ -155,27 +155,31 @@ def rope_and_cache_write(Q, K, V, positions, cos, sin, slots, K_cache, V_cache, 
 # ----------------------------------------------------------------------------------------------
 # norm of every query and key head with the rotation (and the cache append) in one pass
 # ----------------------------------------------------------------------------------------------
-def _check_on(names: str, *tensors) -> int:
-    """All tensors (None is skipped) are CUDA tensors of the first one's device, whose index is returned.
-    ``names``: theirs, separated by spaces, for the message."""
+def _check_on(names: str, required, optional=()) -> int:
+    """All tensors (an optional one may be None) are CUDA tensors of the first one's device, whose index is
+    returned.  ``names``: theirs, separated by spaces, for the message."""
     dev = -1
     try:
-        dev = tensors[0].get_device()
-        for x in tensors:
-            if x is not None and (dev < 0 or x.get_device() != dev):
-                break
-        else:
+        dev = required[0].get_device()
+        same = dev >= 0
+        for x in required:
+            if x.get_device() != dev:
+                same = False
+        for x in optional:
+            if x is not None and x.get_device() != dev:
+                same = False
+        if same:
             return dev
     except AttributeError:          # not a tensor
         pass
-    for x, name in zip(tensors, names.split()):
-        if x is None:
+    for i, (x, name) in enumerate(zip((*required, *optional), names.split())):
+        if x is None and i >= len(required):
             continue
         if not isinstance(x, torch.Tensor) or not x.is_cuda:
             raise RuntimeError(f"{name} must be a CUDA tensor")
         if x.get_device() != dev:
-            raise RuntimeError(f"{name} must be on Q's device, not on {x.device}")
-    raise RuntimeError("Q must be a CUDA tensor")
+            raise RuntimeError(f"{name} must be on the device of the first tensor, not on {x.device}")
+    raise RuntimeError("the tensors must be CUDA tensors of one device")
 
 
 def _contiguous(x, name: str) -> None:
@@ -225,7 +229,7 @@ def _kv_scales(kvd: int, k_scale, v_scale, hkv: int, dev: int) -> None:
         return
     if k_scale is None or v_scale is None:
         raise RuntimeError("FP8 KV needs k_scale and v_scale (float32 [Hkv])")
-    if _check_on("k_scale v_scale", k_scale, v_scale) != dev:
+    if _check_on("k_scale v_scale", (k_scale, v_scale)) != dev:
         raise RuntimeError("k_scale and v_scale must be on Q's device")
     for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
         if t.dtype != torch.float32 or t.numel() != hkv or not t.is_contiguous():
@@ -253,8 +257,8 @@ def _may_overlap(a, b) -> bool:
 
 def _qk_norm_rope(what, Q, K, V, q_weight, k_weight, positions, cos, sin, slots, K_cache, V_cache, head_dim, eps,
                   k_scale, v_scale, out, err_flag):
-    dev = _check_on("Q K V q_weight k_weight positions cos sin slots K_cache V_cache err_flag", Q, K, V, q_weight, k_weight,
-                    positions, cos, sin, slots, K_cache, V_cache, err_flag)
+    dev = _check_on("Q K q_weight k_weight positions cos sin V slots K_cache V_cache err_flag",
+                    (Q, K, q_weight, k_weight, positions, cos, sin), (V, slots, K_cache, V_cache, err_flag))
     if err_flag is not None:
         _flag_word(err_flag)
     dtype = Q.dtype
@@ -321,8 +325,7 @@ def _qk_norm_rope(what, Q, K, V, q_weight, k_weight, positions, cos, sin, slots,
 
 
 def _check_norm_out(Qo, Ko, Q, K, V) -> None:
-    if _check_on("Q out[0] out[1]", Q, Qo, Ko) < 0:
-        raise RuntimeError("out must be CUDA tensors")
+    _check_on("Q out[0] out[1]", (Q, Qo, Ko))
     for t, x, n in ((Qo, Q, "out[0]"), (Ko, K, "out[1]")):
         _rows(t, n)
         if t.shape != x.shape or t.dtype != x.dtype:
@@ -631,12 +634,21 @@ class DecodeStepGraph:
     hold the rotated values.  For the next step the caller appends ``new_slots[b]`` to sequence b's
     slots.  One captured graph serves every step whose cached tokens fit ``max_tokens``.
     With float8 pools pass ``k_scale``/``v_scale`` (float32 ``[Hkv]``).
+
+    ``q_weight``/``k_weight`` (with ``eps``) put the per-head RMS norm in front of the rotation, in the same kernel
+    (:func:`qk_norm_rope_and_cache_write`); ``window`` (with ``n_sinks``) replaces full attention by
+    :func:`paged_window_attention_forward`, whose stale slot-table entries need not be kept up.
     """
 
     def __init__(self, K_cache, V_cache, cos, sin, batch: int, num_heads: int, head_dim: int, max_tokens: int, *,
-                 dtype=None, scale: Optional[float] = None, chunk: Optional[int] = None, k_scale=None, v_scale=None):
+                 dtype=None, scale: Optional[float] = None, chunk: Optional[int] = None, k_scale=None, v_scale=None,
+                 q_weight=None, k_weight=None, eps: float = 1e-6, window: Optional[int] = None, n_sinks: int = 0):
         dev = K_cache.device
         dtype = dtype or (K_cache.dtype if K_cache.dtype in _DT else torch.float16)
+        if (q_weight is None) != (k_weight is None):
+            raise RuntimeError("q_weight and k_weight go together")
+        if window is None and n_sinks:
+            raise RuntimeError("n_sinks needs a window")
         H, D = num_heads, head_dim
         if K_cache.size(1) % D:
             raise RuntimeError("K_cache.size(1) must be a multiple of head_dim")
@@ -656,12 +668,22 @@ class DecodeStepGraph:
         self.chunk = chunk or pick_chunk(batch, Hkv, D, max_tokens, dev, group=H // Hkv, kv_dtype=kvd)
         self.workspace = torch.empty(decode_workspace_bytes(batch, H, D, max_tokens, self.chunk), dtype=torch.uint8,
                                      device=dev)
-        self._keep = (K_cache, V_cache, cos, sin, k_scale, v_scale)
+        self._keep = (K_cache, V_cache, cos, sin, k_scale, v_scale, q_weight, k_weight)
         d = self.dev_in
 
         def step():
-            rope_and_cache_write(d["q"], d["k"], d["v"], d["positions"], cos, sin, d["new_slots"], K_cache, V_cache,
-                                 D, k_scale=k_scale, v_scale=v_scale, err_flag=self.err_flag)
+            if q_weight is not None:
+                qk_norm_rope_and_cache_write(d["q"], d["k"], d["v"], q_weight, k_weight, d["positions"], cos, sin,
+                                             d["new_slots"], K_cache, V_cache, D, eps=eps, k_scale=k_scale, v_scale=v_scale,
+                                             out=(d["q"], d["k"]), err_flag=self.err_flag)
+            else:
+                rope_and_cache_write(d["q"], d["k"], d["v"], d["positions"], cos, sin, d["new_slots"], K_cache, V_cache,
+                                     D, k_scale=k_scale, v_scale=v_scale, err_flag=self.err_flag)
+            if window is not None:
+                paged_window_attention_forward(d["q"], d["k"], d["v"], K_cache, V_cache, d["cache_indices"], d["offsets"], H,
+                                               window, n_sinks, scale=scale, k_scale=k_scale, v_scale=v_scale, out=self.out,
+                                               err_flag=self.err_flag)
+                return
             paged_kv_attention_forward(d["q"], d["k"], d["v"], K_cache, V_cache, d["cache_indices"], d["offsets"], H,
                                        scale=scale, return_sp=False, chunk=self.chunk, k_scale=k_scale,
                                        v_scale=v_scale, workspace=self.workspace, out=self.out,
@@ -913,8 +935,8 @@ def paged_window_attention_forward(Q, K, V, K_cache, V_cache, cache_indices, off
     outside the pools is skipped and sets its bit in ``err_flag``.  One kernel, no workspace.  Returns
     O ``[B, H*D]``.
     """
-    dev = _check_on("Q K V K_cache V_cache cache_indices offsets out err_flag", Q, K, V, K_cache, V_cache, cache_indices, offsets,
-                    out, err_flag)
+    dev = _check_on("Q K V K_cache V_cache cache_indices offsets out err_flag", (Q, K, V, K_cache, V_cache, cache_indices, offsets),
+                    (out, err_flag))
     if err_flag is not None:
         _flag_word(err_flag)
     B, D, Hkv, qd, kvd = _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_scale, dev)
@@ -953,8 +975,8 @@ def paged_window_prefill_attention(Q, K_cache, V_cache, cache_indices, kv_offset
     cores, where a non-finite value in V also reaches the queries of the same 128-row tile that do not see it;
     every other type and head_dim up to 512 runs the generic kernel.  Returns O ``[sum q_len, H*D]``.
     """
-    dev = _check_on("Q K_cache V_cache cache_indices kv_offsets q_offsets out err_flag", Q, K_cache, V_cache, cache_indices, kv_offsets,
-                    q_offsets, out, err_flag)
+    dev = _check_on("Q K_cache V_cache cache_indices kv_offsets q_offsets out err_flag",
+                    (Q, K_cache, V_cache, cache_indices, kv_offsets, q_offsets), (out, err_flag))
     if err_flag is not None:
         _flag_word(err_flag)
     for t, n in ((Q, "Q"), (K_cache, "K_cache"), (V_cache, "V_cache")):
@@ -1008,8 +1030,8 @@ def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, c
     ``shared_prefix_workspace_bytes(...)``) holds nothing between calls; two calls that may overlap need one each.
     A slot outside the pools is skipped and sets its bit in ``err_flag``.  Returns O ``[B, H*D]``.
     """
-    dev = _check_on("Q K V K_cache V_cache prefix_indices cache_indices offsets workspace out err_flag", Q, K, V, K_cache, V_cache,
-                    prefix_indices, cache_indices, offsets, workspace, out, err_flag)
+    dev = _check_on("Q K V K_cache V_cache prefix_indices cache_indices offsets workspace out err_flag",
+                    (Q, K, V, K_cache, V_cache, prefix_indices, cache_indices, offsets), (workspace, out, err_flag))
     if err_flag is not None:
         _flag_word(err_flag)
     B, D, Hkv, qd, kvd = _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_scale, dev)
@@ -1019,13 +1041,13 @@ def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, c
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     P = prefix_indices.numel()
-    need = shared_prefix_workspace_bytes(B, num_heads, Hkv, D, P, scale, qd, kvd)
-    if workspace is None:
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
-    elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
-        raise RuntimeError(f"workspace too small: {need} contiguous bytes needed")
     with _on_index(dev):
+        need = lib.attn_b200_shared_prefix_workspace_bytes(B, num_heads, Hkv, D, P, scale, qd, kvd)
+        if workspace is None:
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
+        elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+            raise RuntimeError(f"workspace too small: {need} contiguous bytes needed")
         check(lib.attn_b200_shared_prefix_decode(
             Q.data_ptr(), K.data_ptr(), V.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), prefix_indices.data_ptr(),
             cache_indices.data_ptr(), offsets.data_ptr(), O.data_ptr(), _ptr(workspace), need, B, num_heads, Hkv, D, P,
