@@ -108,14 +108,14 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
     return x;
 }
 
-// Blocks of query rows of sequence b (window); a sequence whose offsets make no sense has none
+// Blocks of query rows of sequence b (window), -1 if its offsets make no sense
 __device__ __forceinline__ int window_blocks(const AttendParams& p, int b) {
     if (b >= p.B) return 0;
     const int64_t q_beg = b ? p.q_offsets[b - 1] : 0, q_end = p.q_offsets[b];
     const int64_t kv_beg = b ? p.kv_offsets[b - 1] : 0, kv_end = p.kv_offsets[b];
     if (q_beg < 0 || q_end < q_beg || q_end > p.n_q_tokens || kv_beg < 0 || kv_end > p.n_kv_tokens || kv_end - kv_beg < q_end - q_beg) {
         if (p.err_flag) atomicOr(p.err_flag, ATTN_B200_FLAG_BAD_OFFSETS);
-        return 0;
+        return -1;
     }
     const int rows = p.head_pairs ? BM : 2 * BM;
     const int64_t n = (q_end - q_beg + rows - 1) / rows;
@@ -228,7 +228,46 @@ __device__ __forceinline__ bool softmax_rows(SM& sm, int w, uint32_t s_addr, uin
         const bool any_bad = *(volatile int*)&sm.any_bad;
         const uint32_t* const bad = sm.bad[(g0 + j) & 7];
         const int h = min(hi - base, keys - 1), lw = lo - base, s = ns - base;     // in columns of this tile
-        if (keys == BN && !__any_sync(0xffffffffu, any_bad || h < BN - 1 || (lw > 0 && s < BN))) {
+        // Chunks of 32 columns: `dead` ones no row of the warp sees, `whole` ones all rows see, of the others `bits` are
+        // the columns that this row sees.
+        int h_max = BN - 1, h_min = BN - 1, lw_max = 0, lw_min = 0;
+        const bool masked = __any_sync(0xffffffffu, any_bad || h < BN - 1 || (lw > 0 && s < BN));
+        if (masked) {
+            h_max = __reduce_max_sync(0xffffffffu, h);
+            h_min = __reduce_min_sync(0xffffffffu, h);
+            lw_max = __reduce_max_sync(0xffffffffu, lw);
+            lw_min = __reduce_min_sync(0xffffffffu, lw);
+        }
+        auto dead = [&](int c) { return c > h_max || (c + 31 < lw_min && c >= s); };
+        auto whole = [&](int c) { return !any_bad && c + 31 <= h_min && (c >= lw_max || c + 31 < s); };
+        auto bits = [&](int c) -> uint32_t {
+            auto below = [&](int x) { return x <= c ? 0u : x >= c + 32 ? 0xffffffffu : (1u << (x - c)) - 1u; };     // columns < x
+            uint32_t m = below(h + 1) & (~below(lw) | below(s));
+            if (any_bad) m &= ~bad[c >> 5];
+            return m;
+        };
+        if (keys > 96) {
+            if (masked) {
+                // -inf into the columns that are not seen, in tensor memory, before the whole row is read as any other.
+                // (Reading a masked row in chunks, twice, with the dead chunks' exponentials left out took 3 us against
+                // the 1.3 of a row without a mask; this way the main path keeps its registers.)
+#pragma unroll 1
+                for (int c = 0; c < BN; c += 32) {
+                    if (whole(c)) continue;
+                    uint32_t x[32];
+                    if (dead(c)) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] = 0xff800000u;
+                    } else {
+                        tmem_ld32(s_addr + c, reinterpret_cast<float*>(x));
+                        const uint32_t m = bits(c);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] = m >> e & 1u ? x[e] : 0xff800000u;
+                    }
+                    tmem_st32(s_addr + c, x);
+                }
+                tmem_st_wait();
+            }
             float sv[BN];
 #pragma unroll
             for (int c = 0; c < 4; ++c) tmem_ld32_nowait(s_addr + c * 32, sv + c * 32);
@@ -272,21 +311,9 @@ __device__ __forceinline__ bool softmax_rows(SM& sm, int w, uint32_t s_addr, uin
             }
             l += (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
         } else {
-            // A tile at an end of a window, a short first tile, or missing rows: 32 columns at a time, read from tensor
-            // memory for the maximum and again for P.  Chunks that no row of the warp sees (half of the triangles at
-            // both ends) are neither read nor exponentiated, chunks that all rows see are not masked.
-            const int chunks = keys > 96 ? 4 : (keys + 31) / 32;
-            const int h_max = __reduce_max_sync(0xffffffffu, h), h_min = __reduce_min_sync(0xffffffffu, h);
-            const int lw_max = __reduce_max_sync(0xffffffffu, lw), lw_min = __reduce_min_sync(0xffffffffu, lw);
-            auto dead = [&](int c) { return c > h_max || (c + 31 < lw_min && c >= s); };
-            auto whole = [&](int c) { return !any_bad && c + 31 <= h_min && (c >= lw_max || c + 31 < s); };
-            // this row's visible columns of chunk c as bits
-            auto bits = [&](int c) -> uint32_t {
-                auto below = [&](int x) { return x <= c ? 0u : x >= c + 32 ? 0xffffffffu : (1u << (x - c)) - 1u; };     // columns < x
-                uint32_t m = below(h + 1) & (~below(lw) | below(s));
-                if (any_bad) m &= ~bad[c >> 5];
-                return m;
-            };
+            // a short first tile: as many chunks of 32 columns as it has, read from tensor memory for the maximum and
+            // again for P
+            const int chunks = (keys + 31) / 32;
             float mx = -INFINITY;
             for (int c = 0; c < chunks * 32; c += 32) {
                 if (dead(c)) continue;
@@ -407,6 +434,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         sm.box.err_flag = p.err_flag;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (kPrefix && warp == 8 && lane == 0) prefix_item(p, sm.item[0]);
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -663,7 +691,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             // time, once each, so empty and short chunks cost next to nothing.
             int base = 0, mine = 0, upto = 0, before = 0;       // sequences base .. base + 31: blocks of lane's, scan of them, blocks ahead of base
             auto look = [&] {
-                mine = window_blocks(p, base + lane);
+                mine = max(window_blocks(p, base + lane), 0);
                 upto = mine;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
@@ -695,11 +723,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 if (!__all_sync(0xffffffffu, ok)) break;
                 if (lane == 0) {
                     Item& it = sm.item[n % kItems];
-                    it.tiles = 0;
-                    if (!end) {
-                        if constexpr (kPrefix) prefix_item(p, it);
-                        else window_item(p, b, blk, unit, it);
-                    }
+                    if (end) it.tiles = 0;
+                    else if (!kPrefix) window_item(p, b, blk, unit, it);       // (a prefix CTA's is there)
                     mbar_arrive(&sm.item_full[n % kItems]);
                 }
                 if (end) break;
@@ -825,6 +850,37 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
             }
             __syncwarp();
+        } else if (!kPrefix && warp == 11) {
+            // -------------------------------------------------------------- rows that no query tile writes: zeros
+            // past the last sequence, beyond max_q_len, or of a sequence whose offsets are bad; every CTA takes a share
+            const int64_t vecs = (int64_t)p.H * HD / 8;
+            auto zero = [&](int64_t from, int64_t to) {
+                from = from < 0 ? 0 : from;
+                to = to > p.n_q_tokens ? p.n_q_tokens : to;
+                for (int64_t row = from + blockIdx.x; row < to; row += gridDim.x) {
+                    uint4* const dst = reinterpret_cast<uint4*>((T*)p.out + row * p.H * HD);
+                    for (int64_t i = lane; i < vecs; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
+                }
+            };
+            const int64_t covered = (int64_t)p.blocks * (p.head_pairs ? BM : 2 * BM);
+            for (int base = 0; base < p.B; base += 32) {
+                const int b = base + lane;
+                int64_t from = 0, to = 0;
+                if (b < p.B) {
+                    from = b ? p.q_offsets[b - 1] : 0;
+                    to = p.q_offsets[b];
+                    if (window_blocks(p, b) >= 0) {
+                        if (to - from > covered && p.err_flag) atomicOr(p.err_flag, ATTN_B200_FLAG_BAD_OFFSETS);
+                        from += covered;
+                    }
+                }
+                for (unsigned todo = __ballot_sync(0xffffffffu, to > from); todo; todo &= todo - 1) {
+                    const int src = __ffs(todo) - 1;
+                    zero(__shfl_sync(0xffffffffu, from, src), __shfl_sync(0xffffffffu, to, src));
+                }
+            }
+            const int64_t end = p.B ? p.q_offsets[p.B - 1] : 0;
+            zero(end, p.n_q_tokens);
         } else if (!kPrefix && warp == 10) {
             // -------------------------------------------------------------- query tiles
             int uses[2] = {0, 0};
@@ -1003,31 +1059,6 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
 }
 
-// Rows that no query tile writes: past the last sequence, beyond max_q_len, or of a sequence whose offsets are bad.
-__global__ void zero_rows_kernel(void* out, const int32_t* q_offsets, const int32_t* kv_offsets, int B, int64_t n_q, int64_t n_kv, int covered,
-                                 int64_t row_bytes, int32_t* err_flag) {
-    asm volatile("griddepcontrol.launch_dependents;");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t vecs = row_bytes / 16;
-    auto clamped = [&](int64_t v) { return v < 0 ? (int64_t)0 : (v > n_q ? n_q : v); };
-    for (int b = blockIdx.x; b <= B; b += gridDim.x) {
-        const int64_t beg = b ? q_offsets[b - 1] : 0, end = b < B ? q_offsets[b] : n_q;
-        int64_t from = clamped(beg);
-        const int64_t to = clamped(end);
-        if (b < B) {
-            const int64_t kb = b ? kv_offsets[b - 1] : 0, ke = kv_offsets[b];
-            const bool good = beg >= 0 && end >= beg && end <= n_q && kb >= 0 && ke <= n_kv && ke - kb >= end - beg;
-            if (good) {
-                if (end - beg <= covered) continue;
-                if (err_flag && threadIdx.x == 0) atomicOr(err_flag, ATTN_B200_FLAG_BAD_OFFSETS);
-                from = beg + covered;
-            }
-        }
-        uint4* base = reinterpret_cast<uint4*>((char*)out + from * row_bytes);
-        for (int64_t i = threadIdx.x; i < (to - from) * vecs; i += blockDim.x) base[i] = make_uint4(0, 0, 0, 0);
-    }
-}
-
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
@@ -1120,17 +1151,11 @@ int attend_window_launch(AttendParams p, int max_q_len, int D, int dtype, cudaSt
     const int rows = p.head_pairs ? BM : 2 * BM, blocks = (int)(((int64_t)max_q_len + rows - 1) / rows);
     const int units = p.head_pairs ? p.H / 2 : p.H;
     if (p.B > 65535 || units > 65535) return ATTN_B200_ETOOLARGE;
-    if (p.n_q_tokens > 0) {
-        const int rc = launch_dependent(zero_rows_kernel, dim3(p.B < 63 ? p.B + 1 : 64), 256, 0, st, p.out, p.q_offsets, p.kv_offsets, p.B,
-                                        p.n_q_tokens, p.n_kv_tokens, blocks * rows, (int64_t)p.H * D * 2, p.err_flag);
-        if (rc) return rc;
-    }
-    if (blocks == 0 || p.B == 0) return 0;
     p.blocks = blocks;
     p.units = units;
     // one CTA per SM, no more than there can be items
     const int64_t most = (p.n_q_tokens / rows + p.B) * units, sms = current_sm_count();
-    const dim3 grid((unsigned)(most < sms ? most : sms));
+    const dim3 grid((unsigned)(most < 1 ? 1 : most < sms ? most : sms));
     const bool bf = dtype == ATTN_B200_BF16;
     if (D == 64) return bf ? launch<__nv_bfloat16, 64, kWindow, false>(p, grid, st) : launch<__half, 64, kWindow, false>(p, grid, st);
     return bf ? launch<__nv_bfloat16, 128, kWindow, false>(p, grid, st) : launch<__half, 128, kWindow, false>(p, grid, st);

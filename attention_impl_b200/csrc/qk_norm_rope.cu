@@ -158,11 +158,12 @@ __device__ __forceinline__ uint4 ld_once(const void* p) {
 
 template <typename T, int LPH>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
-qk_norm_rope_kernel(const NormRopeParams p) {
+qk_norm_rope_kernel(NormRopeParams p) {
     constexpr int N = Vec<T>::N;
-    // a programmatic dependent (a decode kernel) may be scheduled from here on; it reads nothing this
-    // kernel writes before its own wait
-    asm volatile("griddepcontrol.launch_dependents;");
+    // Launched as a programmatic dependent itself: nothing is read before the kernel ahead has completed.  A dependent
+    // of this kernel (a decode kernel) may be scheduled from here on; it reads nothing written here before its own wait.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tpt = 1 << p.tpt_log2;
     const int tid = threadIdx.x & (tpt - 1);
     const int64_t tok_raw = (int64_t)blockIdx.x * (kThreads >> p.tpt_log2) + (threadIdx.x >> p.tpt_log2);
@@ -375,15 +376,19 @@ template <typename T> int launch(const NormRopeParams& p0, cudaStream_t st) {
         p.tpt_log2 = tl;
         const int64_t per_cta = kThreads >> tl, ctas = (p.n_tokens + per_cta - 1) / per_cta;
         if (ctas > 0x7fffffff) return ATTN_B200_ETOOLARGE;
-        switch (lph) {
-            case 1: qk_norm_rope_kernel<T, 1><<<(unsigned)ctas, kThreads, 0, st>>>(p); break;
-            case 2: qk_norm_rope_kernel<T, 2><<<(unsigned)ctas, kThreads, 0, st>>>(p); break;
-            case 4: qk_norm_rope_kernel<T, 4><<<(unsigned)ctas, kThreads, 0, st>>>(p); break;
-            case 8: qk_norm_rope_kernel<T, 8><<<(unsigned)ctas, kThreads, 0, st>>>(p); break;
-            case 16: qk_norm_rope_kernel<T, 16><<<(unsigned)ctas, kThreads, 0, st>>>(p); break;
-            default: qk_norm_rope_kernel<T, 32><<<(unsigned)ctas, kThreads, 0, st>>>(p); break;
-        }
-        return (int)cudaGetLastError();
+        void (*kernel)(NormRopeParams) = lph == 1 ? qk_norm_rope_kernel<T, 1> : lph == 2 ? qk_norm_rope_kernel<T, 2>
+                                         : lph == 4 ? qk_norm_rope_kernel<T, 4> : lph == 8 ? qk_norm_rope_kernel<T, 8>
+                                         : lph == 16 ? qk_norm_rope_kernel<T, 16> : qk_norm_rope_kernel<T, 32>;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)ctas);
+        cfg.blockDim = dim3(kThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        return (int)cudaLaunchKernelEx(&cfg, kernel, (NormRopeParams)p);
     }
     const int per_token = heads + (p.slots ? p.hk : 0);
     const int64_t items = p.n_tokens * per_token, ctas = (items + 7) / 8;
