@@ -190,9 +190,37 @@ qk_norm_rope_kernel(NormRopeParams p) {
     const T* const q_row = (const T*)p.q + token * p.q_stride;
     const T* const k_row = (const T*)p.k + token * p.k_stride;
     load(q_row, p.hq, grp);
+    // v is only copied; its first chunks are on their way with the first heads of q
+    constexpr int kV = 2;
+    const int v_items = p.slots ? p.hk * hv : 0;
+    const T* const v_row = (const T*)p.v + token * p.v_stride;
+    uint4 uv[kV];
+    auto load_v = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < kV; ++u)
+            if (i0 + u * tpt < v_items) uv[u] = ldg_stream128(v_row + (int64_t)(i0 + u * tpt) * N);
+    };
+    load_v(tid);
     int pos;
     int64_t slot;
     const bool pos_ok = token_ok(p, token, live ? tid : 1, pos, slot);
+    if (slot >= 0 && live) {
+        for (int i0 = tid; i0 < v_items; i0 += tpt * kV) {
+            if (i0 != tid) load_v(i0);
+#pragma unroll
+            for (int u = 0; u < kV; ++u) {
+                const int i = i0 + u * tpt;
+                if (i >= v_items) break;
+                if (p.v_scale) {
+                    float f[N];
+                    Vec<T>::unpack(uv[u], f);
+                    store_pool<T>(p.v_cache, slot * p.hk * p.d + (int64_t)i * N, f, p.v_scale, i / hv);
+                } else {
+                    *reinterpret_cast<uint4*>((T*)p.v_cache + slot * p.hk * p.d + (int64_t)i * N) = uv[u];
+                }
+            }
+        }
+    }
     float2 c[N / 2], s[N / 2];
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) { c[i] = make_float2(1.f, 1.f); s[i] = make_float2(0.f, 0.f); }
@@ -274,28 +302,6 @@ qk_norm_rope_kernel(NormRopeParams p) {
             }
         }
     }
-    if (slot < 0 || !live) return;
-    const int v_items = p.hk * hv;
-    for (int i0 = tid; i0 < v_items; i0 += tpt * 4) {
-        uint4 x[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * tpt;
-            if (i < v_items) x[u] = ldg_stream128((const T*)p.v + token * p.v_stride + (int64_t)i * N);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * tpt;
-            if (i >= v_items) break;
-            if (p.v_scale) {
-                float f[N];
-                Vec<T>::unpack(x[u], f);
-                store_pool<T>(p.v_cache, slot * p.hk * p.d + (int64_t)i * N, f, p.v_scale, i / hv);
-            } else {
-                *reinterpret_cast<uint4*>((T*)p.v_cache + slot * p.hk * p.d + (int64_t)i * N) = x[u];
-            }
-        }
-    }
 }
 
 // Any head_dim, rotary width, stride and alignment: one warp per (token, head); a lane owns the pairs
@@ -367,12 +373,13 @@ template <typename T> int launch(const NormRopeParams& p0, cudaStream_t st) {
         while (lph < slots) lph <<= 1;
         // Threads per token: at least one LPH group, at most the CTA, and few enough that a thread makes
         // kRounds rounds over the q heads, which pays for its coefficients (16384 tokens, 32 + 32 heads of
-        // 128, fp16: 102 us with four rounds, 109 with two, 110 with eight) - unless there are too few
-        // tokens to fill the machine that way (8 tokens: 3.7 us with one round, 7 with four).
+        // 128, fp16: 102 us with four rounds, 109 with two, 110 with eight) - unless the tokens are too few to fill
+        // the machine that way, when each gets as many threads as still make one wave (8 tokens: 3.7 us with one
+        // round, 7 with four; 5000 tokens of 8 + 2 heads: 10.8 us, 14.8 with twice the threads in two waves).
         const int64_t fill = (int64_t)current_sm_count() * kCtasPerSm * kThreads;
         int tl = 0;
         while ((1 << tl) < kThreads && ((1 << tl) < lph || (1 << tl) * kRounds * kUnroll < p.hq * lph)) ++tl;
-        while ((1 << tl) < kThreads && (1 << tl) * kUnroll < p.hq * lph && (p.n_tokens << tl) < fill) ++tl;
+        while ((1 << tl) < kThreads && (1 << tl) * kUnroll < p.hq * lph && (p.n_tokens << (tl + 1)) <= fill) ++tl;
         p.tpt_log2 = tl;
         const int64_t per_cta = kThreads >> tl, ctas = (p.n_tokens + per_cta - 1) / per_cta;
         if (ctas > 0x7fffffff) return ATTN_B200_ETOOLARGE;
