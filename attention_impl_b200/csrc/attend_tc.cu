@@ -207,7 +207,7 @@ __device__ __forceinline__ bool softmax_rows(SM& sm, int w, uint32_t s_addr, uin
                 l *= alpha;
                 if (!mbar_wait(&sm.o_full[w], (c0 + i - 1) & 1, wc)) return false;
                 tc_fence_after();
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < HD / 32; ++c) {
                     float ov[32];
                     tmem_ld32(o_addr + c * 32, ov);
@@ -963,7 +963,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 unsigned char* const stage = (key_split ? sm.k[(last + kStages) % kStages] : sm.q[key_split ? 0 : w]) + (warp & 3) * (kTileBytes / 4);
                 constexpr int kBoxes = kTileBytes / 4 / 4096;                             // boxes that fit the warp's share
                 const bool box = row_w + 32 <= it.n_rows;
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
                     const uint32_t buf = smem_u32(stage) + (c / 32 % kBoxes) * 4096;
                     if (c >= 32 * kBoxes) {
@@ -1000,41 +1000,44 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 float2* const ml = reinterpret_cast<float2*>(p.parts + (int64_t)attend_prefix_parts(p) * rows_all * HD);
                 if (row < it.n_rows) ml[row0 + row] = make_float2(count > 0 ? m : -INFINITY, l);
             } else if (count > 0) {
-                float ov[HD];
-#pragma unroll
-                for (int c = 0; c < HD / 32; ++c) tmem_ld32_nowait(o_addr + c * 32, ov + c * 32);
-                tmem_ld_wait();
-                tc_fence_before();
-                mbar_arrive(&sm.o_free[w]);         // the next item may overwrite the accumulator
                 // a row none of whose keys has a pool row is zero
                 const float inv = m > -INFINITY || l != l ? 1.f / l : 0.f;
                 // A warp's 4 KB of staging hold 64 columns of its 32 rows in the 128-byte-swizzled layout of a TMA box; one
                 // lane stores the box, or, where the chunk ends inside it, the lanes copy the rows that exist.
                 unsigned char* const stage = sm.extra[w] + (warp & 3) * 4096;
+                const uint32_t mine = smem_u32(stage) + lr * 128;
                 const bool box = row_w + 32 <= it.n_rows;
-#pragma unroll
-                for (int c = 0; c < HD; c += 64) {
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");     // the store before has read it
-                    __syncwarp();
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float* o8 = ov + c + e * 8;
-                        st_shared16(smem_u32(stage) + lr * 128 + ((e ^ (lr & 7)) << 4), pack2<T>(o8[0] * inv, o8[1] * inv),
-                                    pack2<T>(o8[2] * inv, o8[3] * inv), pack2<T>(o8[4] * inv, o8[5] * inv), pack2<T>(o8[6] * inv, o8[7] * inv));
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    float ov[32];
+                    tmem_ld32(o_addr + c, ov);
+                    if (c + 32 == HD) {             // the next item may overwrite the accumulator
+                        tc_fence_before();
+                        mbar_arrive(&sm.o_free[w]);
                     }
+                    if (c % 64 == 0) {              // the store before has read the buffer
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        st_shared16(mine + (((e + c / 8 % 8) ^ (lr & 7)) << 4), pack2<T>(ov[8 * e] * inv, ov[8 * e + 1] * inv),
+                                    pack2<T>(ov[8 * e + 2] * inv, ov[8 * e + 3] * inv), pack2<T>(ov[8 * e + 4] * inv, ov[8 * e + 5] * inv),
+                                    pack2<T>(ov[8 * e + 6] * inv, ov[8 * e + 7] * inv));
+                    if (c % 64 == 0) continue;
                     if (box) {
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) {
                             asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
-                                         ::"l"(reinterpret_cast<uint64_t>(&map_o)), "r"(it.head[w] * HD + c), "r"((int)(it.q_beg + row_w)),
+                                         ::"l"(reinterpret_cast<uint64_t>(&map_o)), "r"(it.head[w] * HD + c - 32), "r"((int)(it.q_beg + row_w)),
                                            "r"(smem_u32(stage)) : "memory");
                             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                         }
                     } else {
                         __syncwarp();
                         Rows rows = rows_from(it, w, row_w + lane / 8);
-                        T* const dst = (T*)p.out + c + lane % 8 * 8;
+                        T* const dst = (T*)p.out + c - 32 + lane % 8 * 8;
 #pragma unroll 1
                         for (int i = 0; i < 32; i += 4) {
                             const int rr = i + lane / 8, cc = lane % 8;
