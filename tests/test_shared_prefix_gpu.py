@@ -195,3 +195,22 @@ def test_refusals():
                dict(err_flag=torch.zeros(1, device="cuda"))):
         with pytest.raises(RuntimeError):
             call(**kw)
+
+
+@pytest.mark.parametrize("kv", ["same", "e4m3"])
+def test_tensors_off_the_16_byte_grid(kv):
+    import attention_impl_b200 as A
+    args, more, ref, size, pt, n = _case(200, [20, 0, 30], 4, 2, 128, BF16, kv)
+
+    def shifted(x):
+        buf = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")
+        y = buf[1:].view(x.shape)
+        y.copy_(x)
+        return y
+    for i in range(5):
+        moved = list(args)
+        moved[i] = shifted(args[i])
+        close(A.shared_prefix_attention_forward(*moved, **more), ref, size, BF16, pt, n)
+    out = shifted(args[0])
+    A.shared_prefix_attention_forward(*args, **more, out=out)
+    close(out, ref, size, BF16, pt, n)

@@ -261,3 +261,61 @@ def test_refusals():
     big = torch.zeros(2, 4 * 520, dtype=F16, device="cuda")
     with pytest.raises(RuntimeError, match="head_dim"):
         A.paged_window_attention_forward(big, big, big, big, big, args[5], args[6] * 0, 4, 4)
+
+
+@pytest.mark.parametrize("kv", ["same", "e4m3"])
+def test_tensors_off_the_16_byte_grid(kv):
+    import attention_impl_b200 as A
+    args, more, ref, size, pt, n = _case([70, 200], 4, 2, 128, F16, kv, 90, 4)
+
+    def shifted(x):
+        buf = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")
+        y = buf[1:].view(x.shape)
+        y.copy_(x)
+        return y
+    for i in range(5):
+        moved = list(args)
+        moved[i] = shifted(args[i])
+        close(A.paged_window_attention_forward(*moved, **more), ref, size, F16, pt, n)
+    out = shifted(args[0])
+    A.paged_window_attention_forward(*args, **more, out=out)
+    close(out, ref, size, F16, pt, n)
+
+
+FIRST_CALLS = """
+import torch
+import attention_impl_b200 as A
+D, H = 128, 4
+t = lambda *s: torch.randn(*s, device="cuda").half()
+i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+q, k, kc = t(4, H * D), t(4, 2 * D), t(300, 2 * D)
+w, c = torch.ones(D, device="cuda").half(), torch.ones(64, 64, device="cuda").half()
+table, prefix, off, pos = torch.arange(40, device="cuda").int(), torch.arange(100, 300, device="cuda").int(), i(10, 20, 30, 40), i(0, 1, 2, 3)
+calls = [lambda: A.qk_norm_rope(q, k, w, w, pos, c, c, D)[0],
+         lambda: A.paged_window_attention_forward(q, k, k, kc, kc, table, off, H, 8, 2),
+         None,
+         lambda: A.shared_prefix_attention_forward(q, k, k, kc, kc, prefix, table, off, H)]
+pos1 = pos + 1
+calls[2] = lambda: A.paged_window_prefill_attention(q, kc, kc, table, off, pos1, H, 8, 2, max_q_len=1)
+torch.cuda.synchronize()
+got = []
+for call in calls:                       # the very first call of each is the captured one
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    graph.replay()
+    torch.cuda.synchronize()
+    got.append(out.clone())
+for call, x in zip(calls, got):
+    assert torch.equal(call(), x)
+print("captured first calls agree")
+"""
+
+
+def test_first_call_of_a_process_may_be_a_captured_one():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and "agree" in r.stdout, r.stderr[-2000:]

@@ -219,3 +219,37 @@ def test_refusals():
     big = torch.zeros(2, 4 * 520, dtype=F16, device="cuda")
     with pytest.raises(RuntimeError, match="head_dim"):
         A.paged_window_prefill_attention(big, big, big, args[3], args[4] * 0, args[5] * 0, 4, 4, max_q_len=2)
+
+
+def test_many_sequences():
+    """More sequences than the item list looks at at a time, empty ones and one-token chunks among them, a long tail of
+    rows that belong to nobody."""
+    import attention_impl_b200 as A
+    g = torch.Generator().manual_seed(8)
+    q = [int(x) for x in torch.randint(0, 4, (150,), generator=g)]
+    q[3], q[40], q[149] = 300, 129, 140
+    past = torch.randint(0, 60, (150,), generator=g).tolist()
+    args, ref, size, n = _case(q, past, 2, 1, 64, F16, 40, 3)
+    Q = torch.cat([args[0], torch.full((3000, 128), 7.0, dtype=F16, device="cuda")])
+    out = A.paged_window_prefill_attention(Q, *args[1:], out=torch.full_like(Q, float("nan")))
+    close(out[:sum(q)], ref, size, F16, F16, n)
+    assert (out[sum(q):] == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_tensors_off_the_16_byte_grid(D):
+    import attention_impl_b200 as A
+    args, ref, size, n = _case([50, 200], [30, 0], 4, 2, D, BF16, 70, 4)
+
+    def shifted(x):
+        buf = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")
+        y = buf[1:].view(x.shape)
+        y.copy_(x)
+        return y
+    for i in range(3):
+        moved = list(args)
+        moved[i] = shifted(args[i])
+        close(A.paged_window_prefill_attention(*moved), ref, size, BF16, BF16, n)
+    out = shifted(args[0])
+    A.paged_window_prefill_attention(*args, out=out)
+    close(out, ref, size, BF16, BF16, n)
