@@ -380,6 +380,43 @@ __device__ __forceinline__ bool softmax_rows(SM& sm, int w, uint32_t s_addr, uin
     return true;
 }
 
+// One query row of a window item over again, by a warp, key by key and only the keys it sees.  A tile's V rows are
+// multiplied with P = 0 for the rows that do not see them, and 0 times an infinity or a NaN is a NaN: a row whose
+// result is not finite goes through here, where such a value reaches only the rows that see it.
+template <typename T, int HD>
+__device__ __noinline__ void row_by_itself(const AttendParams& p, const Item& it, int head, int row) {
+    constexpr int E = HD / 32;
+    const int lane = threadIdx.x & 31;
+    const int pos = it.shift + row;
+    const int64_t lo = (int64_t)pos - p.window + 1;
+    const int first = lo > 0 ? (int)lo : 0, sinks = min(p.sinks, first);
+    const int64_t at = ((it.q_beg + row) * p.H + head) * HD;
+    float q[E], o[E], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        q[i] = to_f32<T>(((const T*)p.q)[at + lane + 32 * i]);
+        o[i] = 0.f;
+    }
+    for (int u = 0; u < sinks + pos - first + 1; ++u) {
+        const int slot = p.table[it.beg + (u < sinks ? u : u - sinks + first)];
+        if (slot < 0 || slot >= p.n_slots) continue;
+        const int64_t kv = ((int64_t)slot * p.Hkv + it.hk) * HD + lane;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) s += q[i] * to_f32<T>(((const T*)p.k_cache)[kv + 32 * i]);
+        s = group_sum<32>(s) * p.scale_log2;
+        const float m_new = fmaxf(m, s), sub = m_new > -INFINITY ? m_new : 0.f;
+        const float alpha = fast_exp2(m - sub), pr = fast_exp2(s - sub);
+        l = l * alpha + pr;
+        m = m_new;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] = o[i] * alpha + pr * to_f32<T>(((const T*)p.v_cache)[kv + 32 * i]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < E; ++i) ((T*)p.out)[at + lane + 32 * i] = from_f32<T>(o[i] * inv);
+}
+
 // A window launch is persistent: one CTA per SM takes every gridDim.x-th item, and the item list, the query tiles and
 // the K/V rings run ahead of the softmax, so that the set-up of an item hides under the one before it.  A prefix
 // CTA has one item.
@@ -1007,10 +1044,13 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 unsigned char* const stage = sm.extra[w] + (warp & 3) * 4096;
                 const uint32_t mine = smem_u32(stage) + lr * 128;
                 const bool box = row_w + 32 <= it.n_rows;
+                float probe = 0.f;                  // turns into a NaN where an entry is not finite
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
                     float ov[32];
                     tmem_ld32(o_addr + c, ov);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) probe = fmaf(ov[e], 0.f, probe);
                     if (c + 32 == HD) {             // the next item may overwrite the accumulator
                         tc_fence_before();
                         mbar_arrive(&sm.o_free[w]);
@@ -1048,6 +1088,12 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         }
                         __syncwarp();
                     }
+                }
+                unsigned odd = __ballot_sync(0xffffffffu, probe != 0.f && row < it.n_rows);
+                if (odd) {
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");       // the box is written first
+                    __syncwarp();
+                    for (; odd; odd &= odd - 1) row_by_itself<T, HD>(p, it, it.head[w], row_w + __ffs(odd) - 1);
                 }
             }
             done_with(n);

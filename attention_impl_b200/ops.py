@@ -972,8 +972,9 @@ def paged_window_prefill_attention(Q, K_cache, V_cache, cache_indices, kv_offset
     A slot outside the pools is skipped and sets its bit in ``err_flag``; a query left without any key gives
     zeros, and so do rows of Q that belong to no sequence.  ``max_q_len`` (an upper bound of the chunk
     lengths) avoids the one device->host sync.  float16 and bfloat16 with head_dim 64 or 128 run on the tensor
-    cores, where a non-finite value in V also reaches the queries of the same 128-row tile that do not see it;
-    every other type and head_dim up to 512 runs the generic kernel.  Returns O ``[sum q_len, H*D]``.
+    cores (rows whose result is not finite are computed once more, key by key, so that an infinity or NaN in K or V
+    reaches only the queries that see it); every other type and head_dim up to 512 runs the generic kernel.
+    Returns O ``[sum q_len, H*D]``.
     """
     dev = _check_on("Q K_cache V_cache cache_indices kv_offsets q_offsets out err_flag",
                     (Q, K_cache, V_cache, cache_indices, kv_offsets, q_offsets), (out, err_flag))
@@ -1026,7 +1027,7 @@ def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, c
     possibly empty.  The query of sequence b sees the P prefix tokens, its own tokens and the current one (K, V).
     The prefix's K and V are read once for the batch: the query rows of all sequences are multiplied with them on
     the tensor cores (float16/bfloat16 queries, head_dim 64 or 128, 16-bit or float8 pools).  Other types and head_dims, and
-    prefixes of at most 64 tokens, give the same result with the prefix read per sequence.  ``workspace`` (at least
+    prefixes of at most 64 tokens, give the same result with the prefix read per sequence (``k_scale`` must be positive).  ``workspace`` (at least
     ``shared_prefix_workspace_bytes(...)``) holds nothing between calls; two calls that may overlap need one each.
     A slot outside the pools is skipped and sets its bit in ``err_flag``.  Returns O ``[B, H*D]``.
     """

@@ -349,8 +349,7 @@ ATTN_B200_API int attn_b200_paged_prefill(const void* q, const void* k_cache, co
 /* attn_b200_paged_prefill with a sliding window and sink tokens (no counterpart in the reference): the query at
  * position i of its sequence sees key j iff j <= i and (j > i - window or j < n_sinks), window >= 1.  Slot entries
  * that no query of the call sees are not read.  16-bit types with head_dim 64 or 128 and 0 < scale run on the
- * tensor cores, where a non-finite V value reaches every query of a 128-row tile that has its key in a tile;
- * head_dim up to 512 and F32 run the generic kernel.  A chunk longer than max_q_len or with bad offsets raises
+ * tensor cores; other head_dims up to 512 and F32 run the generic kernel.  A chunk longer than max_q_len or with bad offsets raises
  * ATTN_B200_FLAG_BAD_OFFSETS; rows that are not computed are zero.  A key with an out-of-range slot is skipped
  * (ATTN_B200_FLAG_BAD_SLOT). */
 ATTN_B200_API int attn_b200_paged_window_prefill(const void* q, const void* k_cache, const void* v_cache,

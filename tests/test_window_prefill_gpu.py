@@ -253,3 +253,29 @@ def test_tensors_off_the_16_byte_grid(D):
     out = shifted(args[0])
     A.paged_window_prefill_attention(*args, out=out)
     close(out, ref, size, BF16, BF16, n)
+
+
+@pytest.mark.parametrize("D,dtype", [(128, F16), (64, BF16), (80, F16)])
+def test_not_a_number_reaches_only_who_sees_it(D, dtype):
+    """Infinities and NaN in K and V of tokens that later queries, earlier queries (left behind by the window), or only
+    some heads see."""
+    import attention_impl_b200 as A
+    q, past, H, Hkv, w, s = [200, 90], [40, 10], 4, 2, 50, 3
+    args, *_ = _case(q, past, H, Hkv, D, dtype, w, s)
+    Q, Kc, Vc, table = args[:4]
+    clean = A.paged_window_prefill_attention(*args)
+    t = table.long()
+    for kv_at, pool, value in ((120, Vc, float("inf")), (200, Vc, float("nan")), (130, Kc, float("nan")), (1, Vc, -float("inf"))):
+        row = int(t[kv_at])
+        old = pool[row].clone()
+        pool[row, :D] = value                                  # KV head 0: query heads 0 and 1, sequence 0
+        got = A.paged_window_prefill_attention(*args)
+        pool[row] = old
+        pos = torch.arange(40, 240, device="cuda")
+        sees = (pos >= kv_at) & ((kv_at > pos - w) | (kv_at < s))
+        hit = torch.zeros(290, H * D, dtype=torch.bool, device="cuda")
+        hit[:200][sees, :2 * D] = True
+        assert not torch.isfinite(got[hit]).any() and hit.any()
+        # the others: the same values, to the roundings of P (a row of the tile may have been computed by itself)
+        size = float(Vc[torch.isfinite(Vc).all(1)].abs().max())
+        assert (got[~hit].float() - clean[~hit].float()).abs().max() <= 4 * torch.finfo(dtype).eps / 2 * size
