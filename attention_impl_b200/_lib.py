@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libattn_b200.so")
 
 F16, BF16, F32, E4M3 = 0, 1, 2, 3
 FLAG_BAD_SLOT, FLAG_BAD_POSITION, FLAG_BAD_OFFSETS, FLAG_TIMEOUT = 1, 2, 4, 8
+PREFIX_AUTO, PREFIX_PER_SEQUENCE, PREFIX_TOGETHER = 0, 1, 2
 DECODE_TABLES_READY = 0x100      # or-ed into `stages` of attn_b200_paged_decode
 ABI_VERSION = 4
 STATIC_SCRATCH_BYTES = 16 << 20
@@ -58,9 +59,9 @@ PROTOTYPES = {
                                        _i64, _f32, _i32, _i32, _vp, _vp]),
     "attn_b200_paged_window_prefill": (_i32, [_vp] * 7 + [_i32, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _i32, _i32, _f32, _i32,
                                               _i32, _vp, _vp]),
-    "attn_b200_shared_prefix_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i64, _f32, _i32, _i32]),
+    "attn_b200_shared_prefix_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i64, _f32, _i32, _i32, _i32]),
     "attn_b200_shared_prefix_decode": (_i32, [_vp] * 10 + [_sz, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _f32, _vp, _vp, _i32,
-                                              _i32, _vp, _vp]),
+                                              _i32, _i32, _vp, _vp]),
     "attn_b200_dense_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _f32,
                                          _i32, _vp]),
 }

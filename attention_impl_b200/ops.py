@@ -1010,14 +1010,20 @@ def paged_window_prefill_attention(Q, K_cache, V_cache, cache_indices, kv_offset
     return O
 
 
+def _prefix_how(together: Optional[bool]) -> int:
+    return _lib.PREFIX_AUTO if together is None else _lib.PREFIX_TOGETHER if together else _lib.PREFIX_PER_SEQUENCE
+
+
 def shared_prefix_workspace_bytes(B: int, H: int, Hkv: int, D: int, n_prefix: int, scale: float, q_dtype: int,
-                                  kv_dtype: int) -> int:
-    return lib.attn_b200_shared_prefix_workspace_bytes(B, H, Hkv, D, n_prefix, scale, q_dtype, kv_dtype)
+                                  kv_dtype: int, together: Optional[bool] = None) -> int:
+    """Bytes that :func:`shared_prefix_attention_forward` needs as ``workspace`` (``q_dtype``, ``kv_dtype``: ABI codes)."""
+    return lib.attn_b200_shared_prefix_workspace_bytes(B, H, Hkv, D, n_prefix, scale, q_dtype, kv_dtype, _prefix_how(together))
 
 
 def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, cache_indices, offsets, num_heads: int, *,
                                     scale: Optional[float] = None, k_scale=None, v_scale=None,
-                                    workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                                    together: Optional[bool] = None, workspace: Optional[torch.Tensor] = None,
+                                    out: Optional[torch.Tensor] = None,
                                     err_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`paged_kv_attention_forward` for a batch whose sequences all begin with the same tokens (not in the
     reference).
@@ -1025,9 +1031,10 @@ def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, c
     ``prefix_indices`` int32 ``[P]`` are the pool rows of the shared prefix; ``cache_indices`` int32 ``[T]`` and
     ``offsets`` int32 ``[B]`` (inclusive cumulative) those of every sequence's own cached tokens behind it, either
     possibly empty.  The query of sequence b sees the P prefix tokens, its own tokens and the current one (K, V).
-    The prefix's K and V are read once for the batch: the query rows of all sequences are multiplied with them on
-    the tensor cores (float16/bfloat16 queries, head_dim 64 or 128, 16-bit or float8 pools).  Other types and head_dims, and
-    prefixes of at most 64 tokens, give the same result with the prefix read per sequence (``k_scale`` must be positive).  ``workspace`` (at least
+    ``together=True`` reads the prefix's K and V once for the batch: the query rows of all sequences are multiplied with
+    them on the tensor cores (float16/bfloat16 queries, head_dim 64 or 128, 16-bit or float8 pools with positive
+    ``k_scale``; RuntimeError where that is not so).  ``False`` reads the prefix for every sequence, in one launch.  ``None``
+    (default) chooses: together where it can and the prefix's bytes times the batch are more than 48 MB.  ``workspace`` (at least
     ``shared_prefix_workspace_bytes(...)``) holds nothing between calls; two calls that may overlap need one each.
     A slot outside the pools is skipped and sets its bit in ``err_flag``.  Returns O ``[B, H*D]``.
     """
@@ -1043,7 +1050,8 @@ def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, c
         scale = 1.0 / math.sqrt(D)
     P = prefix_indices.numel()
     with _on_index(dev):
-        need = lib.attn_b200_shared_prefix_workspace_bytes(B, num_heads, Hkv, D, P, scale, qd, kvd)
+        how = _prefix_how(together)
+        need = lib.attn_b200_shared_prefix_workspace_bytes(B, num_heads, Hkv, D, P, scale, qd, kvd, how)
         if workspace is None:
             if need:
                 workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
@@ -1052,7 +1060,7 @@ def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, c
         check(lib.attn_b200_shared_prefix_decode(
             Q.data_ptr(), K.data_ptr(), V.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), prefix_indices.data_ptr(),
             cache_indices.data_ptr(), offsets.data_ptr(), O.data_ptr(), _ptr(workspace), need, B, num_heads, Hkv, D, P,
-            cache_indices.numel(), K_cache.size(0), scale, _ptr(k_scale), _ptr(v_scale), qd, kvd, _ptr(err_flag), _stream()),
+            cache_indices.numel(), K_cache.size(0), scale, _ptr(k_scale), _ptr(v_scale), qd, kvd, how, _ptr(err_flag), _stream()),
             "shared_prefix_attention_forward")
     return O
 

@@ -207,17 +207,20 @@ ATTN_B200_API int attn_b200_paged_window_decode(const void* q, const void* k_new
  * to the current token.  Tensors and types as in attn_b200_paged_decode with block_size 1; n_slots and
  * n_prefix + n_tokens < 2^31.  `workspace`: attn_b200_shared_prefix_workspace_bytes(...) bytes (0: may be NULL),
  * 16-byte aligned, no initialisation, nothing kept between calls; not shared by calls that may overlap.
- * A prefix of more than 64 rows with 16-bit queries, head_dim 64 or 128 and 0 < scale goes through the tensor
- * cores, anything else (head_dim up to 512) reads the prefix per sequence.  k_scale must then be positive. */
+ * `how`: ATTN_B200_PREFIX_TOGETHER multiplies all queries with the prefix on the tensor cores (16-bit queries, head_dim
+ * 64 or 128, 0 < scale and k_scale, 16-byte aligned tensors, a prefix that is not empty; else ATTN_B200_ESHAPE) and needs
+ * the workspace; ATTN_B200_PREFIX_PER_SEQUENCE reads the prefix again for every sequence, in one launch (head_dim up to
+ * 512); ATTN_B200_PREFIX_AUTO takes the first where it can and n_prefix * B rows are more than 48 MB. */
+enum { ATTN_B200_PREFIX_AUTO = 0, ATTN_B200_PREFIX_PER_SEQUENCE = 1, ATTN_B200_PREFIX_TOGETHER = 2 };
 ATTN_B200_API size_t attn_b200_shared_prefix_workspace_bytes(int B, int H, int n_kv_heads, int D, int64_t n_prefix,
-                                                             float scale, int q_dtype, int kv_dtype);
+                                                             float scale, int q_dtype, int kv_dtype, int how);
 ATTN_B200_API int attn_b200_shared_prefix_decode(const void* q, const void* k_new, const void* v_new, const void* k_cache,
                                                  const void* v_cache, const int32_t* prefix_slots, const int32_t* slots,
                                                  const int32_t* offsets, void* out, void* workspace,
                                                  size_t workspace_bytes, int B, int H, int n_kv_heads, int D,
                                                  int64_t n_prefix, int64_t n_tokens, int64_t n_slots, float scale,
                                                  const float* k_scale, const float* v_scale, int q_dtype, int kv_dtype,
-                                                 int32_t* err_flag, void* stream);
+                                                 int how, int32_t* err_flag, void* stream);
 
 /* Same first stage as attn_b200_paged_decode, but the second stage writes, per (b, h), one
  * partial row  [m (log2 domain), l, o[D] (un-normalised)]  of D+2 floats into

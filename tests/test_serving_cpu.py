@@ -57,10 +57,11 @@ def test_window_prefill_arguments():
         assert _prefill(**kw) == want, kw
 
 
-def _shared(B=2, H=4, hkv=2, D=64, P=100, n=10, slots=256, ws=X, ws_bytes=0, ks=None, q=F16, kv=F16, ptr=X, scale=1.0):
+def _shared(B=2, H=4, hkv=2, D=64, P=100, n=10, slots=256, ws=X, ws_bytes=0, ks=None, q=F16, kv=F16, ptr=X, scale=1.0,
+            how=2):
     from attention_impl_b200._lib import lib
     return lib.attn_b200_shared_prefix_decode(ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ws, ws_bytes, B, H, hkv, D, P, n, slots, scale, ks, ks,
-                                              q, kv, None, None)
+                                              q, kv, how, None, None)
 
 
 def test_shared_prefix_arguments():
@@ -68,16 +69,22 @@ def test_shared_prefix_arguments():
     assert _shared(B=0) == 0
     for kw, want in ((dict(B=-1), EINVAL), (dict(hkv=3), EINVAL), (dict(P=-1), EINVAL), (dict(n=-1), EINVAL), (dict(q=E4M3), EDTYPE),
                      (dict(kv=BF16), EDTYPE), (dict(kv=E4M3), EINVAL), (dict(P=1 << 31), ETOOLARGE), (dict(slots=1 << 31), ETOOLARGE),
-                     (dict(ptr=None), EINVAL), (dict(ws=None), EWORKSPACE), (dict(), EWORKSPACE), (dict(ws=X + 4, ws_bytes=1 << 30), EWORKSPACE)):
+                     (dict(ptr=None), EINVAL), (dict(ws=None), EWORKSPACE), (dict(), EWORKSPACE), (dict(ws=X + 4, ws_bytes=1 << 30), EWORKSPACE),
+                     (dict(how=3), EINVAL), (dict(D=80), ESHAPE), (dict(P=0), ESHAPE), (dict(scale=-1.0), ESHAPE), (dict(ptr=X + 2), ESHAPE),
+                     (dict(q=F32, kv=F32), ESHAPE)):
         assert _shared(**kw) == want, kw
     need = lib.attn_b200_shared_prefix_workspace_bytes
-    assert need(2, 4, 2, 64, 64, 1.0, F16, F16) == 0                # read per sequence
-    assert need(2, 4, 2, 64, 100, 1.0, F32, F32) == 0 and need(2, 4, 2, 80, 100, 1.0, F16, F16) == 0
-    assert need(2, 4, 2, 64, 100, -1.0, F16, F16) == 0 and need(0, 4, 2, 64, 100, 1.0, F16, F16) == 0
+    assert need(2, 4, 2, 64, 100, 1.0, F16, F16, 1) == 0            # read per sequence
+    for bad in ((2, 4, 2, 64, 100, 1.0, F32, F32), (2, 4, 2, 80, 100, 1.0, F16, F16), (2, 4, 2, 64, 100, -1.0, F16, F16),
+                (0, 4, 2, 64, 100, 1.0, F16, F16), (2, 4, 2, 64, 0, 1.0, F16, F16)):
+        assert need(*bad, 2) == 0
     # at least one partial set of rows [o[D], m, l], at most two for every key tile
     for B, H, hkv, P in ((2, 4, 2, 100), (64, 32, 8, 32768), (300, 8, 1, 5000)):
-        n = need(B, H, hkv, 128, P, 1.0, F16, E4M3)
+        n = need(B, H, hkv, 128, P, 1.0, F16, E4M3, 2)
         assert n % (B * H * 130 * 4) == 0 and 1 <= n // (B * H * 130 * 4) <= 2 * -(-P // 128)
+    # the choice: bytes of the prefix times the batch above 48 MB, more than one sequence
+    assert need(4, 32, 8, 128, 2048, 1.0, F16, F16, 0) == 0 and need(4, 32, 8, 128, 4096, 1.0, F16, F16, 0) > 0
+    assert need(4, 32, 8, 128, 4096, 1.0, F16, E4M3, 0) == 0 and need(1, 32, 8, 128, 1 << 20, 1.0, F16, F16, 0) == 0
 
 
 def test_host_tensors_are_refused():

@@ -100,8 +100,9 @@ def test_windowed_model_prompts_and_decode_steps(dtype, window, sinks):
         slots = [torch.cat([s, t[None]]) for s, t in zip(slots, new)]
 
 
+@pytest.mark.parametrize("together", [True, False])
 @pytest.mark.parametrize("dtype,kv", [(F16, "same"), (BF16, "e4m3")])
-def test_batch_behind_a_shared_prefix(dtype, kv):
+def test_batch_behind_a_shared_prefix(dtype, kv, together):
     import attention_impl_b200 as A
     m = _Model(dtype, 2)
     (wq, wk), (cos, sin) = m.aux
@@ -127,7 +128,7 @@ def test_batch_behind_a_shared_prefix(dtype, kv):
         rows_k = _wide(Kc.view(torch.uint8)[new].view(pdt) if scales else Kc[new], scales and scales[0])
         m.check_rows(x, pos, qo, rows_k, Vc.view(torch.uint8)[new].view(pdt) if scales else Vc[new], scales)
         table, off = torch.cat(own), torch.tensor([s.numel() for s in own]).cumsum(0)
-        o = A.shared_prefix_attention_forward(qo, ko, v.contiguous(), Kc, Vc, i32(prefix), i32(table), i32(off), H, **sc)
+        o = A.shared_prefix_attention_forward(qo, ko, v.contiguous(), Kc, Vc, i32(prefix), i32(table), i32(off), H, together=together, **sc)
         k64, v64 = _wide(Kc, scales and scales[0]), _wide(Vc, scales and scales[1])
         seqs = [torch.cat([prefix, s]) for s in own]
         ref, size = so.decode(qo.cpu(), ko.cpu(), v.cpu(), [k64[s] for s in seqs], [v64[s] for s in seqs], H, D ** -0.5)

@@ -30,9 +30,12 @@ def _run(*a, **kw):
     import attention_impl_b200 as A
     args, more, ref, size, pt, n = _case(*a, **kw)
     flag = torch.zeros(1, dtype=torch.int32, device="cuda")
-    out = A.shared_prefix_attention_forward(*args, **more, err_flag=flag)
-    assert int(flag) == 0
-    close(out, ref, size, args[0].dtype, pt, n)
+    D, dtype = args[0].size(1) // args[8], args[0].dtype
+    # every way that the case has: read per sequence, multiplied together, and the choice
+    for together in ([True] if args[5].numel() and D in (64, 128) and dtype != F32 else []) + [False, None]:
+        out = A.shared_prefix_attention_forward(*args, **more, err_flag=flag, together=together)
+        assert int(flag) == 0
+        close(out, ref, size, dtype, pt, n)
     return args, more, out
 
 
@@ -80,13 +83,13 @@ def test_prefix_far_below_and_far_above():
     import attention_impl_b200 as A
     D, P, n = 128, 300, 40
     g = torch.Generator().manual_seed(4)
-    for sign in (1, -1):
+    for sign, way in ((1, True), (-1, True), (1, False), (-1, False)):
         q = torch.ones(2, D).half()
         kc = torch.cat([torch.full((P, D), 6.0 * sign), torch.full((n, D), -6.0 * sign)]).half()
         vc = torch.randn(P + n, D, generator=g).half()
         k, v = torch.full((2, D), -6.0 * sign).half(), torch.randn(2, D, generator=g).half()
         out = A.shared_prefix_attention_forward(q.cuda(), k.cuda(), v.cuda(), kc.cuda(), vc.cuda(), torch.arange(P).int().cuda(),
-                                                torch.arange(P, P + n).int().cuda(), torch.tensor([0, n]).int().cuda(), 1)
+                                                torch.arange(P, P + n).int().cuda(), torch.tensor([0, n]).int().cuda(), 1, together=way)
         rows = [torch.arange(P), torch.arange(P + n)]
         ref, size = so.decode(q, k, v, [kc[r] for r in rows], [vc[r] for r in rows], 1, D ** -0.5)
         close(out, ref, size, F16, F16, P + n)
@@ -96,14 +99,15 @@ def test_bf16_queries_of_any_size_over_8_bit_pools():
     import attention_impl_b200 as A
     args, more, *_ = _case(200, [10, 3], 4, 2, 128, BF16, "e4m3")
     args[1] = args[1] * 0
-    a = A.shared_prefix_attention_forward(*args, **more, scale=0.1)
-    for e in (2.0 ** 90, 2.0 ** -90):
-        b = A.shared_prefix_attention_forward(args[0] * e, *args[1:], **more, scale=0.1 / e)
-        assert (a.float() - b.float()).abs().max() <= 2 * 2.0 ** -8 * float(a.abs().max())
+    for way in (True, False):
+        a = A.shared_prefix_attention_forward(*args, **more, scale=0.1, together=way)
+        for e in (2.0 ** 90, 2.0 ** -90):
+            b = A.shared_prefix_attention_forward(args[0] * e, *args[1:], **more, scale=0.1 / e, together=way)
+            assert (a.float() - b.float()).abs().max() <= 2 * 2.0 ** -8 * float(a.abs().max())
 
 
-@pytest.mark.parametrize("D", [128, 80])
-def test_bad_slots_and_offsets(D):
+@pytest.mark.parametrize("D,way", [(128, True), (128, False), (80, False)])
+def test_bad_slots_and_offsets(D, way):
     import attention_impl_b200 as A
     args, more, *_ = _case(300, [20, 30], 4, 2, D, F16)
     Q, K, V, Kc, Vc, prefix, table, off, H = args
@@ -111,7 +115,7 @@ def test_bad_slots_and_offsets(D):
     prefix[[0, 50, 299]] = torch.tensor([-1, Kc.size(0), 2 ** 31 - 1], dtype=torch.int32, device="cuda")
     table[[5, 22]] = -3
     flag = torch.zeros(1, dtype=torch.int32, device="cuda")
-    got = A.shared_prefix_attention_forward(Q, K, V, Kc, Vc, prefix, table, off, H, err_flag=flag)
+    got = A.shared_prefix_attention_forward(Q, K, V, Kc, Vc, prefix, table, off, H, err_flag=flag, together=way)
     assert int(flag) == 1
     ok = lambda t: t[(t >= 0) & (t < Kc.size(0))].cpu().long()  # noqa: E731
     rows = [torch.cat([ok(prefix), ok(table[:20])]), torch.cat([ok(prefix), ok(table[20:])])]
@@ -120,13 +124,13 @@ def test_bad_slots_and_offsets(D):
     close(got, ref, size, F16, F16 if D == 128 else F32, 331)
     # every prefix row missing: the own rows alone
     flag.zero_()
-    got = A.shared_prefix_attention_forward(Q, K, V, Kc, Vc, prefix * 0 - 1, args[6], off, H, err_flag=flag)
+    got = A.shared_prefix_attention_forward(Q, K, V, Kc, Vc, prefix * 0 - 1, args[6], off, H, err_flag=flag, together=way)
     rows = [args[6][:20].cpu().long(), args[6][20:].cpu().long()]
     ref, size = so.decode(Q.cpu(), K.cpu(), V.cpu(), [k64[r] for r in rows], [v64[r] for r in rows], H, D ** -0.5)
     close(got, ref, size, F16, F16 if D == 128 else F32, 31)
     assert int(flag) == 1
     flag.zero_()
-    got = A.shared_prefix_attention_forward(*args[:7], torch.tensor([20, 51], dtype=torch.int32, device="cuda"), H, err_flag=flag)
+    got = A.shared_prefix_attention_forward(*args[:7], torch.tensor([20, 51], dtype=torch.int32, device="cuda"), H, err_flag=flag, together=way)
     assert int(flag) == 4 and torch.isfinite(got).all()
 
 
@@ -143,24 +147,24 @@ def test_nothing_to_do():
 def test_streams_graphs_and_repeats_give_the_same_bits():
     import attention_impl_b200 as A
     args, more, *_ = _case(700, [20, 0, 300, 5], 8, 2, 128, BF16)
-    first = A.shared_prefix_attention_forward(*args)
+    first = A.shared_prefix_attention_forward(*args, together=True)
     for _ in range(5):
-        assert torch.equal(A.shared_prefix_attention_forward(*args), first)
+        assert torch.equal(A.shared_prefix_attention_forward(*args, together=True), first)
     streams = [torch.cuda.Stream() for _ in range(3)]
     outs = [torch.empty_like(first) for _ in streams]
     torch.cuda.synchronize()
     for s, o in zip(streams, outs):
         with torch.cuda.stream(s):
-            A.shared_prefix_attention_forward(*args, out=o)
+            A.shared_prefix_attention_forward(*args, out=o, together=True)
     torch.cuda.synchronize()
     assert all(torch.equal(o, first) for o in outs)
     from attention_impl_b200.ops import shared_prefix_workspace_bytes
-    need = shared_prefix_workspace_bytes(4, 8, 2, 128, 700, 128 ** -0.5, 1, 1)
+    need = shared_prefix_workspace_bytes(4, 8, 2, 128, 700, 128 ** -0.5, 1, 1, True)
     ws = torch.empty(need, dtype=torch.uint8, device="cuda")
     out = torch.zeros_like(first)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        A.shared_prefix_attention_forward(*args, out=out, workspace=ws)
+        A.shared_prefix_attention_forward(*args, out=out, workspace=ws, together=True)
     for _ in range(3):
         out.zero_()
         ws.fill_(255)
@@ -172,13 +176,13 @@ def test_inputs_written_by_the_kernel_ahead():
     """The call is a programmatic dependent of what precedes it: queries and pools written just before."""
     import attention_impl_b200 as A
     args, more, *_ = _case(2000, [64] * 8, 8, 2, 128, F16)
-    want = A.shared_prefix_attention_forward(*args)
+    want = A.shared_prefix_attention_forward(*args, together=True)
     Q, K, V, Kc, Vc = (x.clone() for x in args[:5])
     for _ in range(20):
         for x, y in zip((Kc, Vc, Q, K, V), (args[3], args[4], args[0], args[1], args[2])):
             x.zero_()
             x.copy_(y)
-        assert torch.equal(A.shared_prefix_attention_forward(Q, K, V, Kc, Vc, *args[5:]), want)
+        assert torch.equal(A.shared_prefix_attention_forward(Q, K, V, Kc, Vc, *args[5:], together=True), want)
 
 
 def test_refusals():
@@ -191,10 +195,14 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             call(i, x)
     need = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
-    for kw in (dict(workspace=need[:64]), dict(workspace=need[4:]), dict(out=args[0][:1]), dict(workspace=need.cpu()),
+    for kw in (dict(workspace=need[:64], together=True), dict(workspace=need[4:], together=True), dict(out=args[0][:1]), dict(workspace=need.cpu()),
                dict(err_flag=torch.zeros(1, device="cuda"))):
         with pytest.raises(RuntimeError):
             call(**kw)
+    for bad in (dict(scale=0.0), dict(scale=-1.0), dict(i=5, x=args[5][:0])):
+        call(**bad)
+        with pytest.raises(RuntimeError, match="head_dim"):
+            call(**bad, together=True)
 
 
 @pytest.mark.parametrize("kv", ["same", "e4m3"])
