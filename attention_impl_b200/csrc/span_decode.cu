@@ -231,21 +231,27 @@ __device__ __forceinline__ void fold(const SpanParams& p, FoldWeights& fw, int b
     }
 }
 
-template <int D, bool E4> struct Ring {
+// A warp's ring of kStages tiles (kStages - 1 of them in flight).  Two stages and three CTAs per SM carry a full machine
+// (D = 128, 16 bits, batch 64: 187 us against 207 with three stages and two CTAs); a launch of few CTAs is bound by
+// the latency of its loads and takes as many stages as shared memory has for it.
+template <int D, bool E4, int STAGES> struct Ring {
     static constexpr int kRow = E4 ? D : 2 * D;                  // bytes of a head's K (or V) row
     static constexpr int J = kRow / 64;                          // 16-byte chunks of a row per lane
     static constexpr int kStageBytes = kTile * 2 * kRow;
-    static constexpr int kStages = kStageBytes > 4096 ? 2 : 3;   // D = 128, 16 bits: 3 CTAs of 2 per SM beat 2 of 3 (187 against 207 us, batch 64)
+    static constexpr int kStages = STAGES;
     static constexpr int kWarpBytes = kStages * kStageBytes;
     static constexpr int kBytes = kWarps * kWarpBytes;
-    static constexpr int kCtasPerSm = 227 * 1024 / (kBytes + 4096) < 4 ? 227 * 1024 / (kBytes + 4096) : 4;
+    static constexpr int kFit = 227 * 1024 / (kBytes + 4096);    // CTAs per SM by shared memory
+    static constexpr int kCtasPerSm = kFit < 4 ? kFit : 4;       // and by registers
+    static_assert(kFit >= 1, "shared memory");
     static_assert(kWarpBytes >= 8 * D * 4, "a warp's partial result reuses its ring");
 };
+template <int D, bool E4> constexpr int base_stages() { return kTile * 4 * D / (E4 ? 2 : 1) > 4096 ? 2 : 3; }
 
-template <typename T, int D, bool E4>
-__global__ void __launch_bounds__(kWarps * 32, (Ring<D, E4>::kCtasPerSm))
+template <typename T, int D, bool E4, int STAGES>
+__global__ void __launch_bounds__(kWarps * 32, (Ring<D, E4, STAGES>::kCtasPerSm))
 span_decode_kernel(const SpanParams p) {
-    using R = Ring<D, E4>;
+    using R = Ring<D, E4, STAGES>;
     using MT = typename std::conditional<E4, __half, T>::type;   // e4m3 rows are multiplied as fp16
     using M = Mma16<MT>;
     constexpr int J = R::J, E = E4 ? 4 : 2, CD = E4 ? 16 : 8;    // k-slices and dims per 16-byte chunk
@@ -595,25 +601,32 @@ int launch(K kernel, const SpanParams& p, int64_t units, int smem, cudaStream_t 
     return (int)cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+template <typename T, int D, bool E4, int STAGES>
+int launch_ring(const SpanParams& p, int64_t units, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0};
+    return launch(span_decode_kernel<T, D, E4, STAGES>, p, units, Ring<D, E4, STAGES>::kBytes, st, ready);
+}
+
 template <typename T, int D, bool E4>
 int launch_mma(SpanParams p, int64_t span, bool ragged, cudaStream_t st) {
-    static std::atomic<uint64_t> ready{0};
+    constexpr int kBase = base_stages<D, E4>();
+    using R = Ring<D, E4, kBase>;
     const int G = p.H / p.Hkv;
     p.n_sets = (G + 7) / 8;
     const int vheads = p.Hkv * p.n_sets;
     // Heads per CTA and CTAs per sequence: one wave of CTAs, as full as whole splits make it (a second wave costs a
-    // CTA's whole start and end, ~6 us; a cluster of 16 about 10 more).  Few heads per CTA (several warps to a head)
+    // CTA's whole start and end, ~6 us; a cluster of 16 about 4 more).  Few heads per CTA (several warps to a head)
     // start and end quickest: batch 8, 32 KV heads, 512 tokens 16.9 us with one head per CTA, 18 to 20 with four.  Four
     // adjacent heads read 4 times the contiguous bytes per token, which counts once DRAM is the bound: batch 64, 8 KV
     // heads, 4100 tokens 187 us with four heads and clusters of three, 258 with two, 349 with one.  Sequences of very
     // different lengths want many small CTAs: 64 with 16 to 1024 tokens, 36 us with one head per CTA, 52 with four.
-    const int64_t slots = (int64_t)current_sm_count() * Ring<D, E4>::kCtasPerSm, tiles = (span + kTile - 1) / kTile;
-    const int64_t bytes = (int64_t)p.B * span * 2 * p.Hkv * Ring<D, E4>::kRow;
+    const int64_t slots = (int64_t)current_sm_count() * R::kCtasPerSm, tiles = (span + kTile - 1) / kTile;
+    const int64_t bytes = (int64_t)p.B * span * 2 * p.Hkv * R::kRow;
     auto units_of = [&](int hl) { return (int64_t)p.B * ((vheads + (1 << hl) - 1) >> hl); };
     auto splits_of = [&](int hl) {
         const int64_t fit = slots / units_of(hl), most = (tiles + (kWarps >> hl) - 1) / (kWarps >> hl);
         const int64_t s = fit < most ? fit : most;
-        return s >= 16 ? 16 : s > 8 ? 8 : s < 1 ? 1 : (int)s;
+        return s >= 16 && tiles >= 64 * (kWarps >> hl) ? 16 : s > 8 ? 8 : s < 1 ? 1 : (int)s;     // 16: clusters beyond the portable size
     };
     int hl = 0;
     while (hl < 2 && (2 << hl) <= vheads &&
@@ -623,7 +636,16 @@ int launch_mma(SpanParams p, int64_t span, bool ragged, cudaStream_t st) {
     const int s = splits_of(hl);
     p.hpc_log2 = hl;
     p.splits = s;
-    return launch(span_decode_kernel<T, D, E4>, p, units, Ring<D, E4>::kBytes, st, ready);
+    // the deepest ring that leaves all CTAs resident, where a warp has tiles for it
+    const bool deep = tiles >= 4 * s * (kWarps >> hl);
+    const int64_t per_sm = (units * s + current_sm_count() - 1) / current_sm_count();
+    if constexpr (4 * R::kStageBytes * 6 <= 200 * 1024) {
+        if (deep && per_sm <= Ring<D, E4, 6>::kCtasPerSm) return launch_ring<T, D, E4, 6>(p, units, st);
+    }
+    if constexpr (kBase == 2) {
+        if (deep && per_sm <= Ring<D, E4, 3>::kCtasPerSm) return launch_ring<T, D, E4, 3>(p, units, st);
+    }
+    return launch_ring<T, D, E4, kBase>(p, units, st);
 }
 
 template <typename T, typename KV, int DPL>
@@ -701,8 +723,7 @@ extern "C" int attn_b200_paged_window_decode(const void* q, const void* k_new, c
     p.k_scale = kv_dtype == ATTN_B200_E4M3 ? k_scale : nullptr;
     p.v_scale = kv_dtype == ATTN_B200_E4M3 ? v_scale : nullptr;
     p.err_flag = err_flag;
-    // most sequences are taken to fill the span unless the table shows that they cannot
+    // sequences are taken to be alike: most fill the span, or the table shows that they cannot
     const int64_t seen = (int64_t)window - 1 + n_sinks, average = block_size > 1 ? (int64_t)max_blocks * block_size : n_tokens / B;
-    const bool ragged = B > 1 && average < 2 * seen;
-    return span_decode_launch(p, average < seen ? average + 1 : seen, ragged, q_dtype, kv_dtype, (cudaStream_t)stream);
+    return span_decode_launch(p, average < seen ? average + 1 : seen, false, q_dtype, kv_dtype, (cudaStream_t)stream);
 }
