@@ -630,7 +630,7 @@ int launch_mma(SpanParams p, int64_t span, bool ragged, cudaStream_t st) {
     };
     int hl = 0;
     while (hl < 2 && (2 << hl) <= vheads &&
-           (units_of(hl) > (ragged ? 2 * slots : slots) || (!ragged && bytes > (100 << 20) && splits_of(hl + 1) <= 4)))
+           (units_of(hl) > (ragged ? 2 * slots : slots) || (!ragged && bytes > (100 << 20) && slots / units_of(hl + 1) <= 8)))
         ++hl;
     const int64_t units = units_of(hl);
     const int s = splits_of(hl);
