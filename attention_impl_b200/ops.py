@@ -195,21 +195,19 @@ def _table(x, name: str) -> None:
         raise RuntimeError(f"{name} must be contiguous")
 
 
-class _on_index:
-    """`with torch.cuda.device(index)` that does nothing when it is already current."""
-    __slots__ = ("ctx",)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
-    def __init__(self, index: int):
-        self.ctx = None if index == torch.cuda.current_device() else torch.cuda.device(index)
 
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            return self.ctx.__exit__(*exc)
-        return False
+def _call(fn, what: str, dev: int, *args) -> None:
+    """``fn(*args, stream)`` on device ``dev`` and its current stream; RuntimeError on a status other than 0.  (The device
+    context manager and torch.cuda.current_stream() cost several microseconds; they are taken only when needed.)"""
+    if _current_device() == dev:
+        status = fn(*args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, _stream())
+    if status != 0:
+        check(status, what)
 
 
 def _flag_word(x) -> None:
@@ -217,11 +215,15 @@ def _flag_word(x) -> None:
         raise RuntimeError("err_flag must be an int32 tensor with one entry")
 
 
-def _rows(x, name: str) -> None:
-    """A matrix of whole rows: contiguous columns, rows any distance apart that keeps them disjoint."""
-    if x.dim() != 2 or not (x.is_contiguous() or ((x.size(1) <= 1 or x.stride(1) == 1) and
-                                                  (x.size(0) <= 1 or x.stride(0) >= x.size(1)))):
-        raise RuntimeError(f"{name} must be two-dimensional with contiguous rows that do not overlap")
+def _rows(x, name: str) -> int:
+    """A matrix of whole rows: contiguous columns, rows any distance apart that keeps them disjoint.  Returns the distance."""
+    if x.dim() == 2:
+        if x.is_contiguous():
+            return x.size(1)
+        step, one = x.stride()
+        if (x.size(1) <= 1 or one == 1) and (x.size(0) <= 1 or step >= x.size(1)):
+            return step
+    raise RuntimeError(f"{name} must be two-dimensional with contiguous rows that do not overlap")
 
 
 def _kv_scales(kvd: int, k_scale, v_scale, hkv: int, dev: int) -> None:
@@ -263,8 +265,7 @@ def _qk_norm_rope(what, Q, K, V, q_weight, k_weight, positions, cos, sin, slots,
         _flag_word(err_flag)
     dtype = Q.dtype
     dt = _dtype_code(Q, "Q")
-    _rows(Q, "Q")
-    _rows(K, "K")
+    q_stride, k_stride = _rows(Q, "Q"), _rows(K, "K")
     n_tokens, q_cols = Q.shape
     k_rows, k_cols = K.shape
     if K.dtype != dtype or k_rows != n_tokens:
@@ -293,7 +294,7 @@ def _qk_norm_rope(what, Q, K, V, q_weight, k_weight, positions, cos, sin, slots,
         _table(slots, "slots")
         if slots.numel() != n_tokens:
             raise RuntimeError("slots must have one entry per row of Q")
-        _rows(V, "V")
+        v_stride = _rows(V, "V")
         _contiguous(K_cache, "K_cache")
         _contiguous(V_cache, "V_cache")
         kvd, shape = _kv_code(K_cache, Q), K_cache.shape
@@ -302,11 +303,10 @@ def _qk_norm_rope(what, Q, K, V, q_weight, k_weight, positions, cos, sin, slots,
         if V_cache.dtype != K_cache.dtype:
             raise RuntimeError("K_cache and V_cache must share a dtype")
         _kv_scales(kvd, k_scale, v_scale, hk, dev)
-        n_slots, v_stride = shape[0], V.stride(0)
+        n_slots = shape[0]
     if out is None:
         # contiguous whatever the inputs' strides are: what the attention operators take
-        Qo = torch.empty_like(Q, memory_format=torch.contiguous_format)
-        Ko = torch.empty_like(K, memory_format=torch.contiguous_format)
+        Qo, Ko = _empty_rows(Q, q_stride == q_cols), _empty_rows(K, k_stride == k_cols)
         qo_stride, ko_stride = q_cols, k_cols
     else:
         Qo, Ko = out
@@ -314,14 +314,18 @@ def _qk_norm_rope(what, Q, K, V, q_weight, k_weight, positions, cos, sin, slots,
         qo_stride, ko_stride = Qo.stride(0), Ko.stride(0)
     if n_tokens == 0:
         return Qo, Ko
-    with _on_index(dev):
-        check(lib.attn_b200_qk_norm_rope(
-            Q.data_ptr(), K.data_ptr(), None if V is None else V.data_ptr(), Qo.data_ptr(), Ko.data_ptr(), q_weight.data_ptr(),
-            k_weight.data_ptr(), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ptr(slots), _ptr(K_cache), _ptr(V_cache),
-            n_tokens, q_cols // head_dim, hk, head_dim, cos_shape[1], cos_shape[0], n_slots, Q.stride(0), K.stride(0), v_stride,
-            qo_stride, ko_stride, eps, dt, _DT[w_dtype], _DT[t_dtype], kvd, _ptr(k_scale), _ptr(v_scale), _ptr(err_flag),
-            _stream()), what)
+    _call(lib.attn_b200_qk_norm_rope, what, dev,
+          Q.data_ptr(), K.data_ptr(), None if V is None else V.data_ptr(), Qo.data_ptr(), Ko.data_ptr(), q_weight.data_ptr(),
+          k_weight.data_ptr(), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), None if slots is None else slots.data_ptr(),
+          None if K_cache is None else K_cache.data_ptr(), None if V_cache is None else V_cache.data_ptr(), n_tokens,
+          q_cols // head_dim, hk, head_dim, cos_shape[1], cos_shape[0], n_slots, q_stride, k_stride, v_stride, qo_stride,
+          ko_stride, eps, dt, _DT[w_dtype], _DT[t_dtype], kvd, None if k_scale is None else k_scale.data_ptr(),
+          None if v_scale is None else v_scale.data_ptr(), None if err_flag is None else err_flag.data_ptr())
     return Qo, Ko
+
+
+def _empty_rows(x, contiguous: bool):
+    return torch.empty_like(x) if contiguous else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _check_norm_out(Qo, Ko, Q, K, V) -> None:
@@ -950,12 +954,11 @@ def paged_window_attention_forward(Q, K, V, K_cache, V_cache, cache_indices, off
     O = _output(out, Q)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    with _on_index(dev):
-        check(lib.attn_b200_paged_window_decode(
-            Q.data_ptr(), K.data_ptr(), V.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), cache_indices.data_ptr(),
-            offsets.data_ptr(), O.data_ptr(), B, num_heads, Hkv, D, cache_indices.numel(), K_cache.size(0), block_size,
-            max_blocks, window, n_sinks, scale, _ptr(k_scale), _ptr(v_scale), qd, kvd, _ptr(err_flag), _stream()),
-            "paged_window_attention_forward")
+    _call(lib.attn_b200_paged_window_decode, "paged_window_attention_forward", dev,
+          Q.data_ptr(), K.data_ptr(), V.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), cache_indices.data_ptr(),
+          offsets.data_ptr(), O.data_ptr(), B, num_heads, Hkv, D, cache_indices.numel(), K_cache.size(0), block_size,
+          max_blocks, window, n_sinks, scale, None if k_scale is None else k_scale.data_ptr(),
+          None if v_scale is None else v_scale.data_ptr(), qd, kvd, None if err_flag is None else err_flag.data_ptr())
     return O
 
 
@@ -999,14 +1002,12 @@ def paged_window_prefill_attention(Q, K_cache, V_cache, cache_indices, kv_offset
     O = _output(out, Q)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    with _on_index(dev):
-        if max_q_len is None:
-            max_q_len = max(0, int(torch.diff(q_offsets, prepend=q_offsets.new_zeros(1)).max().item())) if B else 0
-        check(lib.attn_b200_paged_window_prefill(
-            Q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), cache_indices.data_ptr(), kv_offsets.data_ptr(),
-            q_offsets.data_ptr(), O.data_ptr(), B, nq, cache_indices.numel(), min(max_q_len, nq), num_heads, cols // D, D,
-            K_cache.size(0), window, n_sinks, scale, dt, int(force_generic), _ptr(err_flag), _stream()),
-            "paged_window_prefill_attention")
+    if max_q_len is None:
+        max_q_len = max(0, int(torch.diff(q_offsets, prepend=q_offsets.new_zeros(1)).max().item())) if B else 0
+    _call(lib.attn_b200_paged_window_prefill, "paged_window_prefill_attention", dev,
+          Q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), cache_indices.data_ptr(), kv_offsets.data_ptr(),
+          q_offsets.data_ptr(), O.data_ptr(), B, nq, cache_indices.numel(), min(max_q_len, nq), num_heads, cols // D, D,
+          K_cache.size(0), window, n_sinks, scale, dt, int(force_generic), None if err_flag is None else err_flag.data_ptr())
     return O
 
 
@@ -1049,19 +1050,18 @@ def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, c
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     P = prefix_indices.numel()
-    with _on_index(dev):
-        how = _prefix_how(together)
-        need = lib.attn_b200_shared_prefix_workspace_bytes(B, num_heads, Hkv, D, P, scale, qd, kvd, how)
-        if workspace is None:
-            if need:
-                workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
-        elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
-            raise RuntimeError(f"workspace too small: {need} contiguous bytes needed")
-        check(lib.attn_b200_shared_prefix_decode(
-            Q.data_ptr(), K.data_ptr(), V.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), prefix_indices.data_ptr(),
-            cache_indices.data_ptr(), offsets.data_ptr(), O.data_ptr(), _ptr(workspace), need, B, num_heads, Hkv, D, P,
-            cache_indices.numel(), K_cache.size(0), scale, _ptr(k_scale), _ptr(v_scale), qd, kvd, how, _ptr(err_flag), _stream()),
-            "shared_prefix_attention_forward")
+    how = _prefix_how(together)
+    need = lib.attn_b200_shared_prefix_workspace_bytes(B, num_heads, Hkv, D, P, scale, qd, kvd, how)
+    if workspace is None:
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
+    elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+        raise RuntimeError(f"workspace too small: {need} contiguous bytes needed")
+    _call(lib.attn_b200_shared_prefix_decode, "shared_prefix_attention_forward", dev,
+          Q.data_ptr(), K.data_ptr(), V.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), prefix_indices.data_ptr(),
+          cache_indices.data_ptr(), offsets.data_ptr(), O.data_ptr(), None if workspace is None else workspace.data_ptr(), need,
+          B, num_heads, Hkv, D, P, cache_indices.numel(), K_cache.size(0), scale, None if k_scale is None else k_scale.data_ptr(),
+          None if v_scale is None else v_scale.data_ptr(), qd, kvd, how, None if err_flag is None else err_flag.data_ptr())
     return O
 
 
