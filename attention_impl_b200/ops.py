@@ -310,7 +310,7 @@ def _qk_norm_rope(what, Q, K, V, q_weight, k_weight, positions, cos, sin, slots,
         qo_stride, ko_stride = q_cols, k_cols
     else:
         Qo, Ko = out
-        _check_norm_out(Qo, Ko, Q, K, V)
+        _check_norm_out(Qo, Ko, Q, K, V, K_cache, V_cache)
         qo_stride, ko_stride = Qo.stride(0), Ko.stride(0)
     if n_tokens == 0:
         return Qo, Ko
@@ -328,16 +328,16 @@ def _empty_rows(x, contiguous: bool):
     return torch.empty_like(x) if contiguous else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
-def _check_norm_out(Qo, Ko, Q, K, V) -> None:
+def _check_norm_out(Qo, Ko, Q, K, V, K_cache, V_cache) -> None:
     _check_on("Q out[0] out[1]", (Q, Qo, Ko))
     for t, x, n in ((Qo, Q, "out[0]"), (Ko, K, "out[1]")):
         _rows(t, n)
         if t.shape != x.shape or t.dtype != x.dtype:
             raise RuntimeError(f"{n} must have the shape and dtype of its input")
-        for y in (Q, K, V):
+        for y in (Q, K, V, K_cache, V_cache):
             same = y is x and t.data_ptr() == x.data_ptr() and (t.stride(0) == x.stride(0) or x.size(0) <= 1)
             if y is not None and not same and _may_overlap(t, y):
-                raise RuntimeError(f"{n} must be its input itself or share no memory with Q, K and V")
+                raise RuntimeError(f"{n} must be its input itself or share no memory with Q, K, V and the pools")
     if _may_overlap(Qo, Ko):
         raise RuntimeError("out[0] and out[1] must not share memory")
 
@@ -910,12 +910,20 @@ def _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_sca
     return B, D, cols // D, qd, kvd
 
 
-def _output(out, Q):
+def _output(out, Q, *others):
+    """``out``, checked, or a new tensor.  A query row may be read again after its output row is written, and by
+    another CTA, so ``out`` shares no memory with what the call reads."""
     if out is None:
         return torch.empty_like(Q)
     _contiguous(out, "out")
     if out.shape != Q.shape or out.dtype != Q.dtype:
         raise RuntimeError("out must have Q's shape and dtype")
+    begin = out.data_ptr()
+    end = begin + out.numel() * out.element_size()
+    for x in (Q, *others):
+        at = x.data_ptr()
+        if begin < at + x.numel() * x.element_size() and at < end:
+            raise RuntimeError("out must not share memory with Q, K, V or the pools")
     return out
 
 
@@ -951,7 +959,7 @@ def paged_window_attention_forward(Q, K, V, K_cache, V_cache, cache_indices, off
         if block_size < 1 or cache_indices.dim() != 2 or cache_indices.size(0) != B:
             raise RuntimeError("block_size > 1 needs a block table [B, max_blocks]")
         max_blocks = cache_indices.size(1)
-    O = _output(out, Q)
+    O = _output(out, Q, K, V, K_cache, V_cache)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     _call(lib.attn_b200_paged_window_decode, "paged_window_attention_forward", dev,
@@ -999,7 +1007,7 @@ def paged_window_prefill_attention(Q, K_cache, V_cache, cache_indices, kv_offset
     if not cols or cols % D or num_heads % (cols // D) or kv_offsets.numel() != B:
         raise RuntimeError("pools must be [slots, Hkv*D] with Hkv dividing num_heads; one offset per sequence")
     window, n_sinks = _window_args(window, n_sinks)
-    O = _output(out, Q)
+    O = _output(out, Q, K_cache, V_cache)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     if max_q_len is None:
@@ -1034,7 +1042,7 @@ def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, c
     possibly empty.  The query of sequence b sees the P prefix tokens, its own tokens and the current one (K, V).
     ``together=True`` reads the prefix's K and V once for the batch: the query rows of all sequences are multiplied with
     them on the tensor cores (float16/bfloat16 queries, head_dim 64 or 128, 16-bit or float8 pools with positive
-    ``k_scale``; RuntimeError where that is not so).  ``False`` reads the prefix for every sequence, in one launch.  ``None``
+    ``k_scale``; RuntimeError where that is not so, or where the prefix is empty).  ``False`` reads the prefix for every sequence, in one launch.  ``None``
     (default) chooses: together where it can and the prefix's bytes times the batch are more than 48 MB.  ``workspace`` (at least
     ``shared_prefix_workspace_bytes(...)``) holds nothing between calls; two calls that may overlap need one each.
     A slot outside the pools is skipped and sets its bit in ``err_flag``.  Returns O ``[B, H*D]``.
@@ -1046,7 +1054,7 @@ def shared_prefix_attention_forward(Q, K, V, K_cache, V_cache, prefix_indices, c
     B, D, Hkv, qd, kvd = _decode_shapes(Q, K, V, K_cache, V_cache, offsets, num_heads, k_scale, v_scale, dev)
     _table(prefix_indices, "prefix_indices")
     _table(cache_indices, "cache_indices")
-    O = _output(out, Q)
+    O = _output(out, Q, K, V, K_cache, V_cache)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     P = prefix_indices.numel()

@@ -194,7 +194,7 @@ ATTN_B200_API int attn_b200_paged_decode_pick_chunk_gqa(int B, int n_kv_heads, i
  * sequence whose offsets are not non-decreasing or pass n_tokens (or max_blocks*block_size) counts as empty
  * (ATTN_B200_FLAG_BAD_OFFSETS).  head_dim 64, 128, 256 with 16-bit queries run on the tensor cores, other
  * head_dims up to 512 and F32 on the generic kernel.  `slots` has n_tokens entries (block_size 1) or is
- * [B, max_blocks]. */
+ * [B, max_blocks].  `out` overlaps nothing that the call reads. */
 ATTN_B200_API int attn_b200_paged_window_decode(const void* q, const void* k_new, const void* v_new, const void* k_cache,
                                                 const void* v_cache, const int32_t* slots, const int32_t* offsets,
                                                 void* out, int B, int H, int n_kv_heads, int D, int64_t n_tokens,
@@ -206,7 +206,8 @@ ATTN_B200_API int attn_b200_paged_window_decode(const void* q, const void* k_new
  * n_prefix pool rows prefix_slots (read once for the batch), to its own rows slots[offsets[b-1] .. offsets[b]) and
  * to the current token.  Tensors and types as in attn_b200_paged_decode with block_size 1; n_slots and
  * n_prefix + n_tokens < 2^31.  `workspace`: attn_b200_shared_prefix_workspace_bytes(...) bytes (0: may be NULL),
- * 16-byte aligned, no initialisation, nothing kept between calls; not shared by calls that may overlap.
+ * 16-byte aligned, no initialisation, nothing kept between calls; not shared by calls that may overlap.  `out` overlaps
+ * nothing that the call reads.
  * `how`: ATTN_B200_PREFIX_TOGETHER multiplies all queries with the prefix on the tensor cores (16-bit queries, head_dim
  * 64 or 128, 0 < scale and k_scale, 16-byte aligned tensors, a prefix that is not empty; else ATTN_B200_ESHAPE) and needs
  * the workspace; ATTN_B200_PREFIX_PER_SEQUENCE reads the prefix again for every sequence, in one launch (head_dim up to
@@ -354,7 +355,7 @@ ATTN_B200_API int attn_b200_paged_prefill(const void* q, const void* k_cache, co
  * that no query of the call sees are not read.  16-bit types with head_dim 64 or 128 and 0 < scale run on the
  * tensor cores; other head_dims up to 512 and F32 run the generic kernel.  A chunk longer than max_q_len or with bad offsets raises
  * ATTN_B200_FLAG_BAD_OFFSETS; rows that are not computed are zero.  A key with an out-of-range slot is skipped
- * (ATTN_B200_FLAG_BAD_SLOT). */
+ * (ATTN_B200_FLAG_BAD_SLOT).  `out` overlaps nothing that the call reads. */
 ATTN_B200_API int attn_b200_paged_window_prefill(const void* q, const void* k_cache, const void* v_cache,
                                                  const int32_t* slots, const int32_t* kv_offsets,
                                                  const int32_t* q_offsets, void* out, int B, int64_t n_q_tokens,

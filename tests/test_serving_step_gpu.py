@@ -144,3 +144,26 @@ def test_step_graph_arguments():
     for kw in (dict(q_weight=wq), dict(k_weight=wk), dict(n_sinks=2), dict(window=0)):
         with pytest.raises(RuntimeError):
             A.DecodeStepGraph(Kc, Vc, cos, sin, 2, H, D, 32, **kw)
+
+
+def test_outputs_apart_from_what_is_read():
+    """An output that shares memory with the queries, the new token's rows or a pool is refused; a neighbour is not."""
+    import attention_impl_b200 as A
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    buf = torch.randn(12, HKV * D, device="cuda").to(F16)
+    Q, K, V, out, Kc, Vc = buf[:2], buf[2:4], buf[4:6], buf[6:8], buf[8:10], buf[10:12]
+    calls = (lambda o: A.paged_window_attention_forward(Q, K, V, Kc, Vc, i32([0, 1]), i32([1, 2]), HKV, 4, out=o),
+             lambda o: A.shared_prefix_attention_forward(Q, K, V, Kc, Vc, i32([0]), i32([1]), i32([0, 1]), HKV, out=o),
+             lambda o: A.paged_window_prefill_attention(Q, Kc, Vc, i32([0, 1]), i32([1, 2]), i32([1, 2]), HKV, 4, out=o, max_q_len=1))
+    for n, call in enumerate(calls):
+        want = call(None)
+        assert torch.equal(call(out), want)
+        for o in (Q, buf[1:3], Kc, Vc, buf[7:9]) + (() if n == 2 else (K, V, buf[5:7])):
+            with pytest.raises(RuntimeError, match="share memory"):
+                call(o)
+    pos, tab, w = i32([0, 1]), torch.ones(2, D // 2, device="cuda", dtype=F16), torch.ones(D, device="cuda", dtype=F16)
+    norm = lambda o: A.qk_norm_rope_and_cache_write(Q, K, V, w, w, pos, tab, tab, pos, Kc, Vc, D, out=o)  # noqa: E731
+    for o in ((out, Kc), (Vc, K), (buf[9:11], K)):
+        with pytest.raises(RuntimeError, match="share no memory"):
+            norm(o)
+    norm((out, K))
