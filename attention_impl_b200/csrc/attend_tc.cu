@@ -35,10 +35,12 @@ constexpr int kSub = 128 * 128;                 // bytes of a [128 rows x 64 ele
 constexpr int kItems = 4;                       // items published ahead
 // Warps 0-3 and 4-7 softmax, 8 item list, 9 MMA thread, 10 query tiles; 12-15 K and V, 32 rows of a tile each.  With
 // e4m3 rows 12-13 and 14-15 turn the raw K and V rows into fp16.
-// Registers per thread: setmaxnreg draws on the 512 * 128 that the CTA was launched with.
+// Registers per thread: setmaxnreg draws on the 512 * 128 that the CTA was launched with.  The softmax warps fit their row of
+// 128 scores in 184; what the MMA thread and the gather warps spill counts more, for all others wait for them (four prompts: 303
+// us with 184 / 88 / 56, 317 with 184 / 72 / 72, 332 with 208 / 56 / 40).
 constexpr int kThreads = 512;
 template <bool E4> struct Cfg {
-    static constexpr int kSoftmax = E4 ? 200 : 208, kOther = E4 ? 48 : 56, kGather = E4 ? 64 : 40;
+    static constexpr int kSoftmax = 184, kOther = E4 ? 72 : 88, kGather = E4 ? 72 : 56;
     static_assert(8 * 32 * kSoftmax + 4 * 32 * kOther + 4 * 32 * kGather <= kThreads * 128, "register pool");
 };
 
