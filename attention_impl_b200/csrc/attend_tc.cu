@@ -293,8 +293,8 @@ __device__ __forceinline__ bool softmax_rows(SM& sm, int w, uint32_t s_addr, uin
                     float x0, x1, x2, x3, p0, p1, p2, p3;
                     fma2(x0, x1, sv[c * 64 + e], sv[c * 64 + e + 1], scale, scale, nm, nm);
                     fma2(x2, x3, sv[c * 64 + e + 2], sv[c * 64 + e + 3], scale, scale, nm, nm);
-                    // all on the special-function unit: with two of eight as a cubic on the FMA pipe, which the packed
-                    // prefill gains from, four prompts took 403 us instead of 380 (issue slots, not the unit, are short here)
+                    // all on the special-function unit: with two of sixteen as a cubic on the FMA pipe, which the packed
+                    // prefill gains from, four prompts took 312 us instead of 306 (issue slots, not the unit, are short here)
                     p0 = fast_exp2(x0);
                     p1 = fast_exp2(x1);
                     p2 = fast_exp2(x2);
@@ -1046,13 +1046,16 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 unsigned char* const stage = sm.extra[w] + (warp & 3) * 4096;
                 const uint32_t mine = smem_u32(stage) + lr * 128;
                 const bool box = row_w + 32 <= it.n_rows;
-                float probe = 0.f;                  // turns into a NaN where an entry is not finite
+                float probe = 0.f, probe2 = 0.f;    // turn into a NaN where an entry is not finite
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
                     float ov[32];
                     tmem_ld32(o_addr + c, ov);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) probe = fmaf(ov[e], 0.f, probe);
+                    for (int e = 0; e < 32; e += 2) {
+                        fma2(probe, probe2, ov[e], ov[e + 1], 0.f, 0.f, probe, probe2);
+                        fma2(ov[e], ov[e + 1], ov[e], ov[e + 1], inv, inv, -0.f, -0.f);
+                    }
                     if (c + 32 == HD) {             // the next item may overwrite the accumulator
                         tc_fence_before();
                         mbar_arrive(&sm.o_free[w]);
@@ -1063,9 +1066,9 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        st_shared16(mine + (((e + c / 8 % 8) ^ (lr & 7)) << 4), pack2<T>(ov[8 * e] * inv, ov[8 * e + 1] * inv),
-                                    pack2<T>(ov[8 * e + 2] * inv, ov[8 * e + 3] * inv), pack2<T>(ov[8 * e + 4] * inv, ov[8 * e + 5] * inv),
-                                    pack2<T>(ov[8 * e + 6] * inv, ov[8 * e + 7] * inv));
+                        st_shared16(mine + (((e + c / 8 % 8) ^ (lr & 7)) << 4), pack2<T>(ov[8 * e], ov[8 * e + 1]),
+                                    pack2<T>(ov[8 * e + 2], ov[8 * e + 3]), pack2<T>(ov[8 * e + 4], ov[8 * e + 5]),
+                                    pack2<T>(ov[8 * e + 6], ov[8 * e + 7]));
                     if (c % 64 == 0) continue;
                     if (box) {
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1091,7 +1094,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         __syncwarp();
                     }
                 }
-                unsigned odd = __ballot_sync(0xffffffffu, probe != 0.f && row < it.n_rows);
+                unsigned odd = __ballot_sync(0xffffffffu, probe + probe2 != 0.f && row < it.n_rows);
                 if (odd) {
                     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");       // the box is written first
                     __syncwarp();
